@@ -40,6 +40,8 @@ typedef struct det_event det_event_t;
 typedef struct det_graph det_graph_t;
 typedef struct det_kv det_kv_t;
 typedef struct det_scratch det_scratch_t;
+typedef struct det_rope_table det_rope_table_t;
+typedef struct det_adapters det_adapters_t;
 
 /* ------------------------------------------------------------------------ */
 /* Context, memory, timing                                                   */
@@ -150,6 +152,165 @@ int det_argmax_first_noalloc(det_ctx_t* ctx, const int32_t* x_dev, uint64_t n, u
 #define DET_EW_SCALE 2    /* x = scale_act(x, scalar) */
 #define DET_EW_SOFTCAP 3  /* x = softcap_act(x, scalar) */
 int det_elementwise(det_ctx_t* ctx, int op, int32_t* x_dev, const int32_t* y_dev, uint64_t n, int32_t scalar);
+
+/* ------------------------------------------------------------------------ */
+/* Verifying drafted tokens for many requests                                */
+/* ------------------------------------------------------------------------ */
+/* Four operators that one verification step of a serving batch runs one after
+ * the other; no counterpart in the reference, which decodes one token of one
+ * request per call. Their arithmetic is that of the primitives above, so a
+ * drafted token that is accepted has the bits that decoding it would give.
+ * They are enqueued on the context stream, allocate nothing once their scratch
+ * has grown to a call's size (run a call once before capturing it), and do not
+ * synchronize. Device arrays are read when the work runs: words in them that
+ * are out of range (ids, spans, starts) select nothing, as described below.
+ * Outputs must not overlap inputs except where a call says so. */
+
+/* Rotation tables: the frequencies of rope_rotate_pairs_in_place
+ * (det_num/ops.rs:151-196), computed once on the host. */
+#define DET_ROPE_HALF 0        /* pair i is (i, i + rotary_dim / 2): det_rope's layout */
+#define DET_ROPE_INTERLEAVED 1 /* pair i is (2 i, 2 i + 1) */
+#define DET_ROPE_SCALE_NONE 0
+#define DET_ROPE_SCALE_LINEAR 1 /* every frequency f becomes g = f / factor */
+#define DET_ROPE_SCALE_RAMP 2   /* w f + (1 - w) g, w = clamp((t - low_turns) / (high_turns - low_turns), 0, 1) of the
+                                   t = original_positions f / (2 pi) turns over the original context */
+typedef struct det_rope_spec {
+  uint64_t rotary_dim;    /* rotated leading part of a head (even, may be 0) */
+  uint64_t freq_base_dim; /* even, at least 2 */
+  int64_t base_acc;       /* Q32.32, above 0 and below i64::MAX */
+  int32_t layout;
+  int32_t scaling;
+  int64_t factor_acc; /* Q32.32, at least 1 (LINEAR, RAMP) */
+  int64_t low_turns_acc, high_turns_acc; /* Q32.32, 0 <= low < high (RAMP) */
+  uint64_t original_positions;           /* 1 .. 2^32 (RAMP) */
+  int32_t amplitude; /* Q16.16 above 0: sine and cosine are multiplied by it (65536: as they are) */
+} det_rope_spec_t;
+/* Quotients and products are rounded half to even in Q32.32 (turns: from the
+ * exact original_positions * f). */
+int det_rope_table_create(det_ctx_t* ctx, const det_rope_spec_t* spec, det_rope_table_t** out);
+void det_rope_table_free(det_rope_table_t* table);
+
+/* Head norms and rotation in one pass. Each set is rows x heads head rows of
+ * head_dim values, row r at x_dev + r * stride (heads * head_dim of them),
+ * written to out_dev + r * out_stride; out_dev may be x_dev with the same
+ * stride. DET_HEAD_NORM applies rms_norm_in_place with gain_dev [head_dim], or
+ * value_rms_norm_in_place without gain (det_num/ops.rs:95-131); then
+ * DET_HEAD_ROTATE rotates the pairs by position positions_dev[r] (position 0:
+ * the identity, times the amplitude); a set without flags is copied. With an
+ * amplitude other than 1 every rotated pair's cosine and sine are
+ * mul_sat(c, amplitude), mul_sat(s, amplitude). table and positions_dev may be
+ * NULL when no set rotates. head_dim up to 1024, at most 4 sets. */
+#define DET_HEAD_NORM 1u
+#define DET_HEAD_ROTATE 2u
+typedef struct det_head_rows {
+  const int32_t* x_dev;
+  uint64_t stride;
+  uint64_t heads;
+  const int32_t* gain_dev;
+  int32_t* out_dev;
+  uint64_t out_stride;
+  uint32_t flags;
+} det_head_rows_t;
+int det_head_norm_rope(det_ctx_t* ctx, const det_rope_table_t* table, const uint32_t* positions_dev, uint64_t rows,
+                       uint64_t head_dim, int64_t eps_acc, const det_head_rows_t* sets, uint64_t n_sets);
+
+/* One sequence's cached key and value rows: row r (0 <= r < rows) at
+ * k_dev + p * stride, p = first + r, less wrap past a ring's end (wrap 0: a
+ * linear cache; else first < wrap and rows <= wrap). */
+typedef struct det_attn_cache {
+  const int32_t* k_dev;
+  const int32_t* v_dev;
+  uint64_t stride;
+  uint64_t rows;
+  uint64_t first;
+  uint64_t wrap;
+} det_attn_cache_t;
+/* The rows of a layer's cache handle as such a view, valid until the cache
+ * takes more tokens or is freed; fails without det data. */
+int det_kv_view(const det_kv_t* kv, det_attn_cache_t* out);
+/* Host only: the masks and depths of a tree of n (at most 64) drafted rows.
+ * parents[i] < i is a row's parent, -1 for a child of the last cached row;
+ * masks[i] has row i's own bit and its ancestors', depths[i] counts the
+ * ancestors (a row's position is the cached length + its depth). */
+int det_tree_masks(const int32_t* parents, uint64_t n, uint64_t* masks, uint32_t* depths);
+
+/* Attention of drafted rows over caches (attention_output_into,
+ * det_kernels.rs:340-367, over each row's visible rows). Sequence b has
+ * drafts[b] (0 .. 64) drafted rows; q [total][num_heads * head_dim] at
+ * q_stride, k and v [total][num_kv_heads * head_dim] at kv_stride, out like q
+ * at out_stride, all sequences' rows one after the other. Row i sees, in this
+ * order, the cached rows starts_dev[i] .. rows - 1 of its sequence (starts_dev
+ * NULL: all) and the drafted rows j of its sequence whose bit j of masks_dev[i]
+ * is set (bits past drafts[b] are ignored). A row that sees nothing gives
+ * zeros. head_dim up to 512, at most 1048576 cached rows. caches and drafts are
+ * host arrays, read before the call returns. */
+int det_attention_tree(det_ctx_t* ctx, const det_attn_cache_t* caches, const uint32_t* drafts, uint64_t n_sequences,
+                       const int32_t* q_dev, uint64_t q_stride, const int32_t* k_dev, const int32_t* v_dev,
+                       uint64_t kv_stride, const uint64_t* masks_dev, const uint32_t* starts_dev, uint64_t num_heads,
+                       uint64_t num_kv_heads, uint64_t head_dim, int32_t* out_dev, uint64_t out_stride);
+
+/* Low-rank adapters of one projection (rows x cols): adapter i adds
+ * scale_act(B (A x), scale) to the projection's row, A = down [rank][cols] and
+ * B = up [rows][rank], stored as det_matrix_upload stores them (element width
+ * 8 with a row scale, 16 or 32; both products requantized as det_linear's).
+ * rank 1 .. 256. */
+typedef struct det_adapter_spec {
+  uint64_t rank;
+  int32_t down_width;
+  const void* down;
+  const int32_t* down_scale;
+  int32_t up_width;
+  const void* up;
+  const int32_t* up_scale;
+  int32_t scale; /* Q16.16 */
+} det_adapter_spec_t;
+#define DET_NO_ADAPTER 0xffffffffu
+int det_adapters_create(det_ctx_t* ctx, uint64_t rows, uint64_t cols, const det_adapter_spec_t* specs, uint64_t n,
+                        det_adapters_t** out);
+void det_adapters_free(det_adapters_t* adapters);
+/* det_linear_slab of m rows with the adapter of each: out[t] =
+ * add_sat(W x_t, scale_act(B_i (A_i x_t), scale_i)), i = adapter_dev[t]; a row
+ * whose i is not an adapter's (DET_NO_ADAPTER) is W x_t. */
+int det_linear_adapters(det_ctx_t* ctx, const det_matrix_t* w, const det_adapters_t* adapters, uint64_t m,
+                        const int32_t* act_dev, const uint32_t* adapter_dev, int32_t* out_dev);
+
+/* Decoding rules of n rows of logits; every pointer is a device array and may
+ * be NULL (no such rule). In this order:
+ *  - penalties [n]: a token that occurs c > 0 times in the row's history first
+ *    becomes div_act(x, repetition) if x > 0, else mul_sat(x, repetition)
+ *    (repetition 65536, or 0 and below: unchanged), then loses c * frequency +
+ *    presence (Q16.16 each);
+ *  - biases: entry e of bias_begin[r] .. bias_begin[r + 1] - 1 adds
+ *    bias_values[e] to token bias_ids[e] (entries of one token add up); the
+ *    penalties and biases of a token are summed in 64 bits and saturated once;
+ *  - mask [n][mask_stride words]: a token whose bit (token % 32 of word
+ *    token / 32) is clear becomes i32::MIN and cannot be chosen.
+ * The history of row r is the ids of its spans_per_row spans [begin, end) =
+ * spans[r][s][0..1] into ids [n_ids] (rows may share spans; ends past n_ids
+ * are cut there, as bias_begin is at n_bias); ids of vocab and above are ignored. */
+typedef struct det_penalties {
+  int32_t repetition, frequency, presence;
+} det_penalties_t;
+typedef struct det_logit_rules {
+  const det_penalties_t* penalties_dev;
+  const uint32_t* ids_dev;
+  uint64_t n_ids;
+  const uint32_t* spans_dev;
+  uint64_t spans_per_row;
+  const uint32_t* bias_begin_dev;
+  const uint32_t* bias_ids_dev;
+  const int32_t* bias_values_dev;
+  uint64_t n_bias;
+  const uint32_t* mask_dev;
+  uint64_t mask_stride;
+} det_logit_rules_t;
+#define DET_NO_TOKEN 0xffffffffu
+/* Applies the rules (NULL: none) to logits [n][vocab] at `stride`, writes the
+ * results to out_dev at out_stride (NULL: not written; may be logits_dev with
+ * the same stride) and each row's first maximum among the tokens that the mask
+ * leaves to tokens_dev (NULL: not wanted; DET_NO_TOKEN when it leaves none). */
+int det_select_tokens(det_ctx_t* ctx, const int32_t* logits_dev, uint64_t n, uint64_t vocab, uint64_t stride,
+                      const det_logit_rules_t* rules, int32_t* out_dev, uint64_t out_stride, uint32_t* tokens_dev);
 
 /* ------------------------------------------------------------------------ */
 /* Model: Gemma4TransformerModel in det mode (gemma/io.rs:1043-1123)         */

@@ -31,6 +31,7 @@
 #include "audit.h"
 #include "commit.h"
 #include "kernels.h"
+#include "verify.h"
 
 using det::DevMatrix;
 
@@ -84,6 +85,7 @@ struct det_ctx {
   Scratch<int64_t> gemm_planes;  // K-range partial planes of split GEMMs
   Scratch<void> attn_work;       // work area of the MFMA form of causal attention
   Scratch<void> rows_work;       // activation rows of a session's prefill (PrefillRows)
+  Scratch<void> verify_work;     // of the operators that verify drafted tokens
   bool capturing = false;        // between det_ctx_capture_begin and _end
   std::vector<DevRef> recorded;  // scratch objects of the calls recorded since then
 
@@ -144,6 +146,10 @@ struct det_ctx {
     a.work_bytes = attn_work.bytes;
   }
   void ensure_rows_work(size_t bytes) { grow(rows_work, bytes, "prefill row"); }
+  void* verify_scratch(size_t bytes) {
+    grow(verify_work, bytes, "verification");
+    return verify_work.get();
+  }
   // Slab GEMM / GEMV dispatch: int8 weights with at least kGemmMinRows
   // activation rows take the MFMA GEMM, everything else the GEMV kernels.
   static constexpr uint64_t kGemmMinRows = 16;
@@ -193,6 +199,24 @@ struct det_ctx {
 struct det_matrix {
   det_ctx* ctx = nullptr;
   DevMatrix m;
+};
+
+// Inverse frequencies of one rotation (Q32.32) on the device.
+struct det_rope_table {
+  det_ctx* ctx = nullptr;
+  DevRef freq;
+  uint32_t pairs = 0;
+  bool interleaved = false;
+  int32_t amplitude = 0;
+};
+// The adapters of one projection: each one's A as a matrix, its packed B.
+struct det_adapters {
+  det_ctx* ctx = nullptr;
+  uint64_t rows = 0, cols = 0, kpad = 0;
+  uint32_t n = 0, max_rank = 0;
+  std::vector<DevMatrix> down;
+  std::vector<DevRef> up;
+  DevRef table;  // det::DevAdapter[n]
 };
 
 struct det_event {
@@ -3269,6 +3293,98 @@ int64_t* noalloc_parts_on(int device) {
 }  // namespace
 
 // ---------------------------------------------------------------------------
+// Verifying drafted tokens
+// ---------------------------------------------------------------------------
+namespace {
+
+// Makes the context's device current for a call, whatever the caller's is.
+struct OnDevice {
+  int was = -1;
+  explicit OnDevice(const det_ctx* ctx) {
+    int cur = 0;
+    HIPC(hipGetDevice(&cur));
+    if (cur == ctx->device) return;
+    HIPC(hipSetDevice(ctx->device));
+    was = cur;
+  }
+  ~OnDevice() {
+    if (was >= 0) (void)hipSetDevice(was);
+  }
+};
+
+DevRef to_device(det_ctx* ctx, const void* src, size_t bytes) {
+  DevRef d = dev_alloc(std::max<size_t>(bytes, 1));
+  if (bytes) {
+    HIPC(hipMemcpyAsync(d.get(), src, bytes, hipMemcpyHostToDevice, ctx->stream));
+    HIPC(hipStreamSynchronize(ctx->stream));
+  }
+  return d;
+}
+
+// round(n / d) ties to even of 128-bit n >= 0, d > 0, at most i64::MAX
+int64_t quotient_rte(unsigned __int128 n, unsigned __int128 d) {
+  unsigned __int128 q = n / d;
+  const unsigned __int128 r = n - q * d;
+  if (r > d - r || (r == d - r && (q & 1))) ++q;
+  return q > (unsigned __int128)(INT64_MAX) ? INT64_MAX : int64_t(q);
+}
+
+std::vector<int64_t> rope_frequencies(const det_rope_spec_t& sp) {
+  using u128 = unsigned __int128;
+  const uint64_t pairs = sp.rotary_dim / 2;
+  std::vector<int64_t> f(pairs);
+  det::rope_inv_freq_table(sp.base_acc, uint32_t(sp.freq_base_dim), uint32_t(pairs), f.data());
+  if (sp.scaling == DET_ROPE_SCALE_NONE) return f;
+  constexpr uint64_t kTwoPi = 26986075409ull;  // 2 pi in Q32.32
+  for (int64_t& x : f) {
+    const int64_t g = quotient_rte(u128(uint64_t(x)) << 32, uint64_t(sp.factor_acc));
+    if (sp.scaling == DET_ROPE_SCALE_LINEAR) {
+      x = g;
+      continue;
+    }
+    // turns over the original context; past every ramp when they pass i64
+    const u128 turned = u128(sp.original_positions) * uint64_t(x);
+    const int64_t turns = turned >> 95 ? INT64_MAX : quotient_rte(turned << 32, kTwoPi);
+    int64_t w = 0;
+    if (turns >= sp.high_turns_acc) w = det::kOneAcc;
+    else if (turns > sp.low_turns_acc)
+      w = quotient_rte(u128(uint64_t(turns - sp.low_turns_acc)) << 32, uint64_t(sp.high_turns_acc - sp.low_turns_acc));
+    x = det::add_sat64(det::acc_mul(w, x), det::acc_mul(det::kOneAcc - w, g));
+  }
+  return f;
+}
+
+// B's rows in the layout of det::DevAdapter, from the tile-major upload.
+DevRef pack_up(det_ctx* ctx, const DevMatrix& M, size_t* scale_at, size_t* sum_at) {
+  const HostDigits h = untile(ctx, M);
+  const uint64_t tiles = (h.rows + 15) / 16, kg = (h.cols + 15) / 16, planes = uint64_t(h.planes);
+  const size_t q_bytes = round_up(tiles * planes * kg * 256, 256);
+  *scale_at = q_bytes;
+  *sum_at = q_bytes + tiles * 16 * 4;
+  std::vector<uint8_t> buf(q_bytes + 2 * tiles * 16 * 4, 0);
+  int32_t* scale = reinterpret_cast<int32_t*>(buf.data() + *scale_at);
+  int32_t* sum = reinterpret_cast<int32_t*>(buf.data() + *sum_at);
+  for (uint64_t r = 0; r < h.rows; ++r) {
+    scale[r] = h.scale[r];
+    int64_t s = 0;
+    for (uint64_t p = 0; p < planes; ++p)
+      for (uint64_t c = 0; c < h.cols; ++c) {
+        const int8_t d = h.d[(p * h.rows + r) * h.cols + c];
+        buf[(((r >> 4) * planes + p) * kg + c / 16) * 256 + (r & 15) * 16 + c % 16] = uint8_t(d);
+        s += int64_t(d) * (int64_t(1) << (8 * p));
+      }
+    sum[r] = int32_t(s);  // (within int32 by the row-mass bound)
+  }
+  return to_device(ctx, buf.data(), buf.size());
+}
+
+void need_rows(uint64_t stride, uint64_t width, const char* what) {
+  if (stride < width) bail(std::string(what) + " rows overlap: the stride is below the row's width");
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------------------
 // C ABI
 // ---------------------------------------------------------------------------
 namespace {
@@ -3374,7 +3490,8 @@ int det_ctx_capture_end(det_ctx_t* ctx, det_graph_t** out) {
     ctx->capturing = false;
     auto g = std::make_unique<det_graph>();
     g->scratch.swap(ctx->recorded);
-    for (const DevRef& r : {ctx->limbs.mem, ctx->gemm_a.mem, ctx->gemm_planes.mem, ctx->attn_work.mem})
+    for (const DevRef& r : {ctx->limbs.mem, ctx->gemm_a.mem, ctx->gemm_planes.mem, ctx->attn_work.mem,
+                            ctx->verify_work.mem})
       if (r) g->scratch.push_back(r);
     HIPC(hipStreamEndCapture(ctx->stream, &g->graph));
     HIPC(hipGraphInstantiate(&g->exec, g->graph, nullptr, nullptr, 0));
@@ -3517,6 +3634,307 @@ int det_elementwise(det_ctx_t* ctx, int op, int32_t* x, const int32_t* y, uint64
         break;
       default: bail("unknown elementwise op");
     }
+  });
+}
+
+int det_rope_table_create(det_ctx_t* ctx, const det_rope_spec_t* spec, det_rope_table_t** out) {
+  if (!ctx) {
+    g_error = "context is required";
+    return 1;
+  }
+  return guarded(ctx, [&] {
+    if (!spec || !out) bail("a rotation spec and an output handle are required");
+    const det_rope_spec_t& sp = *spec;
+    if (ctx->capturing) bail("det_ctx capture: a rotation table cannot be created inside a capture");
+    if (sp.rotary_dim % 2) contract("rope_rotate_pairs requires an even rotary_dim");
+    if (sp.rotary_dim > det::kHeadMaxDim) bail("rotary_dim above " + std::to_string(det::kHeadMaxDim) + " is not supported");
+    if (sp.freq_base_dim < 2 || sp.freq_base_dim % 2)
+      contract("rope_rotate_pairs requires an even freq_base_dim of at least 2");
+    if (sp.freq_base_dim > UINT32_MAX) bail("freq_base_dim should fit in u32");
+    if (sp.base_acc <= 0) contract("rope_rotate_pairs requires a positive base");
+    if (sp.base_acc == INT64_MAX) contract("nth_root_acc: attempt to add with overflow (RoPE base i64::MAX)");
+    if (sp.layout != DET_ROPE_HALF && sp.layout != DET_ROPE_INTERLEAVED) bail("unknown rotation layout");
+    if (sp.scaling < DET_ROPE_SCALE_NONE || sp.scaling > DET_ROPE_SCALE_RAMP) bail("unknown rotation scaling");
+    if (sp.scaling != DET_ROPE_SCALE_NONE && sp.factor_acc < det::kOneAcc) bail("the scaling factor is below 1");
+    if (sp.scaling == DET_ROPE_SCALE_RAMP &&
+        (sp.low_turns_acc < 0 || sp.high_turns_acc <= sp.low_turns_acc || sp.original_positions == 0 ||
+         sp.original_positions > uint64_t(1) << 32))
+      bail("the scaling ramp requires 0 <= low_turns < high_turns and 1 to 2^32 original positions");
+    if (sp.amplitude <= 0) bail("the rotation's amplitude must be above 0");
+    OnDevice on(ctx);
+    const std::vector<int64_t> f = rope_frequencies(sp);
+    auto t = std::make_unique<det_rope_table>();
+    t->ctx = ctx;
+    t->pairs = uint32_t(sp.rotary_dim / 2);
+    t->interleaved = sp.layout == DET_ROPE_INTERLEAVED;
+    t->amplitude = sp.amplitude;
+    t->freq = to_device(ctx, f.data(), f.size() * 8);
+    *out = t.release();
+  });
+}
+void det_rope_table_free(det_rope_table_t* t) {
+  if (!t) return;
+  (void)hipStreamSynchronize(t->ctx->stream);
+  delete t;
+}
+int det_head_norm_rope(det_ctx_t* ctx, const det_rope_table_t* table, const uint32_t* positions, uint64_t rows,
+                       uint64_t hd, int64_t eps, const det_head_rows_t* sets, uint64_t n_sets) {
+  if (!ctx) {
+    g_error = "context is required";
+    return 1;
+  }
+  return guarded(ctx, [&] {
+    if (n_sets == 0 || n_sets > det::kHeadSets || !sets) bail("one to four sets of head rows are required");
+    if (hd == 0) contract("rms_norm requires a non-empty input slice");
+    if (hd > det::kHeadMaxDim) bail("head_dim above " + std::to_string(det::kHeadMaxDim) + " is not supported");
+    if (rows > INT32_MAX) bail("too many rows");
+    det::HeadRopeArgs a{};
+    bool rotates = false;
+    uint64_t total = 0;
+    for (uint64_t i = 0; i < n_sets; ++i) {
+      const det_head_rows_t& h = sets[i];
+      if (h.flags & ~(DET_HEAD_NORM | DET_HEAD_ROTATE)) bail("unknown head row flags");
+      if (h.heads > (uint64_t(1) << 20)) bail("too many heads");
+      if (h.heads == 0 || rows == 0) continue;
+      if (!h.x_dev || !h.out_dev) bail("head rows and their output are required");
+      need_rows(h.stride, h.heads * hd, "head");
+      need_rows(h.out_stride, h.heads * hd, "output head");
+      if (h.x_dev == h.out_dev && h.stride != h.out_stride) bail("head rows in place require one stride");
+      if ((h.flags & DET_HEAD_NORM) && eps < 0) contract("rms_norm_scale requires a non-negative epsilon");
+      rotates = rotates || (h.flags & DET_HEAD_ROTATE);
+      a.set[a.n_sets++] = {h.x_dev, h.out_dev, h.gain_dev, h.stride, h.out_stride, uint32_t(h.heads), h.flags};
+      total += h.heads;
+    }
+    if (rotates) {
+      if (!table || !positions) bail("rotated head rows require a rotation table and positions");
+      if (table->ctx != ctx) bail("the rotation table belongs to another context");
+      if (2 * uint64_t(table->pairs) > hd) contract("rope_rotate_pairs requires rotary_dim to fit within the input width");
+      a.pairs = table->pairs;
+      a.interleaved = table->interleaved;
+      a.amplitude = table->amplitude;
+      a.freq = static_cast<const int64_t*>(table->freq.get());
+      a.positions = positions;
+      if (ctx->capturing) ctx->recorded.push_back(table->freq);
+    }
+    if (a.n_sets == 0) return;
+    a.hd = uint32_t(hd);
+    a.total = uint32_t(total);
+    a.eps = eps;
+    a.rows = rows;
+    OnDevice on(ctx);
+    det::launch_head_rope(a, ctx->stream);
+    HIPC(hipGetLastError());
+  });
+}
+
+int det_kv_view(const det_kv_t* kv, det_attn_cache_t* out) {
+  if (!kv) {
+    g_error = "cache is required";
+    return 1;
+  }
+  return guarded(kv->ctx, [&] {
+    const GKv& c = kv->c;
+    if (!out) bail("an output view is required");
+    if (!c.has) bail("cache holds no det data");
+    *out = {c.k, c.v, c.row_w, c.len, c.ring ? c.start : 0, c.ring ? c.cap : 0};
+  });
+}
+int det_tree_masks(const int32_t* parents, uint64_t n, uint64_t* masks, uint32_t* depths) {
+  return guarded(nullptr, [&] {
+    if (n > det::kTreeMaxDrafts) bail("a tree has at most 64 drafted rows");
+    if (n && (!parents || !masks || !depths)) bail("parents, masks and depths are required");
+    for (uint64_t i = 0; i < n; ++i) {
+      const int32_t p = parents[i];
+      if (p < -1 || (p >= 0 && uint64_t(p) >= i)) bail("a drafted row's parent must come before it");
+      masks[i] = (p < 0 ? 0 : masks[p]) | uint64_t(1) << i;
+      depths[i] = p < 0 ? 0 : depths[p] + 1;
+    }
+  });
+}
+int det_attention_tree(det_ctx_t* ctx, const det_attn_cache_t* caches, const uint32_t* drafts, uint64_t n_seq,
+                       const int32_t* q, uint64_t q_stride, const int32_t* k, const int32_t* v, uint64_t kv_stride,
+                       const uint64_t* masks, const uint32_t* starts, uint64_t nh, uint64_t nkv, uint64_t hd,
+                       int32_t* out, uint64_t out_stride) {
+  if (!ctx) {
+    g_error = "context is required";
+    return 1;
+  }
+  return guarded(ctx, [&] {
+    if (nkv == 0 || nh < nkv || nh % nkv) bail("invalid Gemma head configuration");
+    if (nh > 4096) bail("too many heads");
+    if (hd == 0) bail("empty attention problem");
+    if (hd > 512) bail("head_dim above 512 is not supported");
+    if (n_seq && (!caches || !drafts)) bail("caches and drafted row counts are required");
+    if (n_seq > (uint64_t(1) << 20)) bail("too many sequences");
+    std::vector<det::TreeSeq> seqs;
+    seqs.reserve(n_seq);
+    uint64_t total = 0;
+    for (uint64_t b = 0; b < n_seq; ++b) {
+      const det_attn_cache_t& c = caches[b];
+      if (drafts[b] > det::kTreeMaxDrafts) bail("a sequence has at most 64 drafted rows");
+      if (c.rows > det::kTreeMaxRows) bail("caches of more than 1048576 rows are not supported");
+      if (drafts[b] == 0) continue;
+      if (c.rows) {
+        if (!c.k_dev || !c.v_dev) bail("cached rows are required");
+        need_rows(c.stride, nkv * hd, "cached");
+        if (c.wrap ? (c.first >= c.wrap || c.rows > c.wrap) : c.first > UINT64_MAX / 2)
+          bail("a ring cache requires first < wrap and rows <= wrap");
+      }
+      seqs.push_back({c.k_dev, c.v_dev, c.stride, c.first, c.wrap, uint32_t(c.rows), drafts[b], total});
+      total += drafts[b];
+    }
+    if (total == 0) return;
+    if (!q || !k || !v || !masks || !out) bail("drafted rows, their masks and an output are required");
+    need_rows(q_stride, nh * hd, "query");
+    need_rows(out_stride, nh * hd, "output");
+    need_rows(kv_stride, nkv * hd, "drafted");
+    det::TreeArgs a{};
+    a.q = q; a.k = k; a.v = v; a.masks = masks; a.starts = starts; a.out = out;
+    a.q_ld = q_stride; a.kv_ld = kv_stride; a.out_ld = out_stride;
+    a.nh = uint32_t(nh); a.nkv = uint32_t(nkv); a.groups = uint32_t(nh / nkv); a.hd = uint32_t(hd);
+    OnDevice on(ctx);
+    void* work = ctx->verify_scratch(det::tree_work_bytes(a, seqs.data(), uint32_t(seqs.size())));
+    det::launch_tree_attention(a, seqs.data(), uint32_t(seqs.size()), work, ctx->stream);
+    HIPC(hipGetLastError());
+  });
+}
+
+int det_adapters_create(det_ctx_t* ctx, uint64_t rows, uint64_t cols, const det_adapter_spec_t* specs, uint64_t n,
+                        det_adapters_t** out) {
+  if (!ctx) {
+    g_error = "context is required";
+    return 1;
+  }
+  det_adapters* raw = nullptr;
+  const int st = guarded(ctx, [&] {
+    if (!out) bail("an output handle is required");
+    if (ctx->capturing) bail("det_ctx capture: adapters cannot be created inside a capture");
+    if (rows == 0 || cols == 0) bail("an empty projection has no adapters");
+    if (cols > 130000) bail("adapters of more than 130000 columns are not supported");
+    if (rows > UINT32_MAX) bail("too many rows");
+    if (n == 0 || n > 65536 || !specs) bail("1 to 65536 adapters are required");
+    OnDevice on(ctx);
+    raw = new det_adapters;
+    raw->ctx = ctx;
+    raw->rows = rows;
+    raw->cols = cols;
+    raw->kpad = round_up(cols, 128);
+    raw->n = uint32_t(n);
+    std::vector<det::DevAdapter> table;
+    for (uint64_t i = 0; i < n; ++i) {
+      const det_adapter_spec_t& sp = specs[i];
+      if (sp.rank == 0 || sp.rank > det::kAdapterMaxRank)
+        bail("an adapter's rank must be 1 to " + std::to_string(det::kAdapterMaxRank));
+      if (!sp.down || !sp.up) bail("null adapter values");
+      raw->down.push_back(upload_matrix(ctx, sp.rank, cols, sp.down_width, sp.down, sp.down_scale));
+      const DevMatrix& A = raw->down.back();
+      DevMatrix B = upload_matrix(ctx, rows, sp.rank, sp.up_width, sp.up, sp.up_scale);
+      size_t scale_at = 0, sum_at = 0;
+      DevRef up;
+      try {
+        up = pack_up(ctx, B, &scale_at, &sum_at);
+      } catch (...) {
+        free_matrix(B);
+        throw;
+      }
+      const uint32_t b_planes = uint32_t(B.planes);
+      free_matrix(B);
+      raw->up.push_back(up);
+      const int8_t* p = static_cast<const int8_t*>(up.get());
+      det::DevAdapter d{};
+      d.a = A.q, d.a_scale = A.scale, d.a_rowsum = A.rowsum, d.a_planes = uint32_t(A.planes);
+      d.b = p, d.b_scale = reinterpret_cast<const int32_t*>(p + scale_at);
+      d.b_rowsum = reinterpret_cast<const int32_t*>(p + sum_at), d.b_planes = b_planes;
+      d.rank = uint32_t(sp.rank), d.kg = uint32_t((sp.rank + 15) / 16), d.scale = sp.scale;
+      table.push_back(d);
+      raw->max_rank = std::max(raw->max_rank, d.kg * 16);
+    }
+    raw->table = to_device(ctx, table.data(), table.size() * sizeof(table[0]));
+    *out = raw;
+  });
+  if (st) det_adapters_free(raw);
+  return st;
+}
+void det_adapters_free(det_adapters_t* ad) {
+  if (!ad) return;
+  (void)hipStreamSynchronize(ad->ctx->stream);
+  for (DevMatrix& m : ad->down) free_matrix(m);
+  delete ad;
+}
+int det_linear_adapters(det_ctx_t* ctx, const det_matrix_t* w, const det_adapters_t* ad, uint64_t m,
+                        const int32_t* act, const uint32_t* index, int32_t* out) {
+  if (!ctx) {
+    g_error = "context is required";
+    return 1;
+  }
+  return guarded(ctx, [&] {
+    if (!w || !ad) bail("a projection and its adapters are required");
+    if (ad->ctx != ctx || w->ctx != ctx) bail("the projection or its adapters belong to another context");
+    if (w->m.rows != ad->rows || w->m.cols != ad->cols) bail("the adapters belong to a projection of another shape");
+    if (m == 0) return;
+    if (m > (uint64_t(1) << 24)) bail("too many rows");
+    if (!act || !index || !out) bail("activation rows, adapter indexes and an output are required");
+    OnDevice on(ctx);
+    det::AdapterArgs a{};
+    a.set = static_cast<const det::DevAdapter*>(ad->table.get());
+    a.n = ad->n;
+    a.max_rank = ad->max_rank;
+    a.index = index;
+    a.act = act;
+    a.m = m, a.cols = ad->cols, a.kpad = ad->kpad, a.rows = ad->rows;
+    a.out = out;
+    void* work = ctx->verify_scratch(det::adapter_work_bytes(a));
+    ctx->linear(w->m, act, m, w->m.cols, out, w->m.rows, nullptr);
+    det::launch_adapters(a, work, ctx->stream);
+    HIPC(hipGetLastError());
+  });
+}
+
+int det_select_tokens(det_ctx_t* ctx, const int32_t* logits, uint64_t n, uint64_t vocab, uint64_t stride,
+                      const det_logit_rules_t* rules, int32_t* out, uint64_t out_stride, uint32_t* tokens) {
+  if (!ctx) {
+    g_error = "context is required";
+    return 1;
+  }
+  return guarded(ctx, [&] {
+    if (vocab == 0) contract("argmax_first requires a non-empty slice");
+    if (vocab >= UINT32_MAX) bail("the vocabulary should fit in u32");
+    if (n > 65535) bail("at most 65535 rows of logits");
+    if (n == 0) return;
+    if (!logits) bail("logits are required");
+    if (!out && !tokens) bail("an output or a token array is required");
+    need_rows(stride, vocab, "logit");
+    det::SelectArgs a{};
+    if (out) {
+      need_rows(out_stride, vocab, "output");
+      if (out == logits && out_stride != stride) bail("logits in place require one stride");
+    }
+    a.logits = logits, a.ld = stride, a.n = n, a.vocab = vocab;
+    if (rules) {
+      const det_logit_rules_t& r = *rules;
+      constexpr uint64_t kMost = uint64_t(1) << 28;
+      if (r.n_ids > kMost || r.n_bias > kMost) bail("at most 268435456 history ids and biases");
+      if (r.penalties_dev && r.spans_per_row) {
+        if (r.spans_per_row > 8) bail("a row's history has at most 8 spans");
+        if (!r.spans_dev || (r.n_ids && !r.ids_dev)) bail("penalties require the history's spans and ids");
+        a.penalties = reinterpret_cast<const det::SelectPenalty*>(r.penalties_dev);
+        a.ids = r.ids_dev, a.n_ids = r.n_ids, a.spans = r.spans_dev, a.spans_per_row = uint32_t(r.spans_per_row);
+      }
+      if (r.bias_begin_dev && r.n_bias) {
+        if (!r.bias_ids_dev || !r.bias_values_dev) bail("biases require their ids and values");
+        a.bias_begin = r.bias_begin_dev, a.bias_ids = r.bias_ids_dev, a.bias_values = r.bias_values_dev;
+        a.n_bias = r.n_bias;
+      }
+      if (r.mask_dev) {
+        if (r.mask_stride < (vocab + 31) / 32) bail("the mask's rows have fewer bits than the vocabulary");
+        a.mask = r.mask_dev, a.mask_ld = r.mask_stride;
+      }
+    }
+    a.out = out, a.out_ld = out_stride, a.tokens = tokens;
+    OnDevice on(ctx);
+    void* work = ctx->verify_scratch(det::select_work_bytes(a));
+    det::launch_select(a, work, ctx->stream);
+    HIPC(hipGetLastError());
   });
 }
 

@@ -26,6 +26,10 @@ DET_EW_ADD, DET_EW_GELU_MUL, DET_EW_SCALE, DET_EW_SOFTCAP = 0, 1, 2, 3
 DET_COMMIT_NONE, DET_COMMIT_ACTIVATIONS, DET_COMMIT_KV, DET_COMMIT_ALL = 0, 1, 2, 3
 DET_DECODE_PER_OP = 0x100
 DET_DECODE_EAGER = 0x200
+DET_ROPE_HALF, DET_ROPE_INTERLEAVED = 0, 1
+DET_ROPE_SCALE_NONE, DET_ROPE_SCALE_LINEAR, DET_ROPE_SCALE_RAMP = 0, 1, 2
+DET_HEAD_NORM, DET_HEAD_ROTATE = 1, 2
+DET_NO_ADAPTER = DET_NO_TOKEN = 0xFFFFFFFF
 
 
 class DetError(RuntimeError):
@@ -144,6 +148,104 @@ class Sampling(C.Structure):
                 ("has_temperature", C.c_int32), ("temperature", C.c_float),
                 ("has_top_k", C.c_int32), ("top_k", C.c_uint64),
                 ("has_top_p", C.c_int32), ("top_p", C.c_float)]
+
+
+class RopeSpec(C.Structure):
+    """det_rope_spec_t: a rotation's frequencies, layout and long-context scaling."""
+
+    _fields_ = [("rotary_dim", C.c_uint64), ("freq_base_dim", C.c_uint64), ("base_acc", C.c_int64),
+                ("layout", C.c_int32), ("scaling", C.c_int32), ("factor_acc", C.c_int64),
+                ("low_turns_acc", C.c_int64), ("high_turns_acc", C.c_int64), ("original_positions", C.c_uint64),
+                ("amplitude", C.c_int32)]
+
+
+def _dev(buf) -> Optional[int]:
+    return None if buf is None else buf.ptr
+
+
+class HeadRows(C.Structure):
+    """det_head_rows_t: rows x heads head rows of one call of Context.head_norm_rope.
+
+    ``out`` None writes in place; ``gain`` None with ``norm`` is the value norm."""
+
+    _fields_ = [("x_dev", C.c_void_p), ("stride", C.c_uint64), ("heads", C.c_uint64), ("gain_dev", C.c_void_p),
+                ("out_dev", C.c_void_p), ("out_stride", C.c_uint64), ("flags", C.c_uint32)]
+
+    def __init__(self, x, stride: int, heads: int, out=None, out_stride: int | None = None, gain=None,
+                 norm: bool = True, rotate: bool = True):
+        super().__init__(_dev(x), stride, heads, _dev(gain), _dev(x if out is None else out),
+                         stride if out_stride is None else out_stride,
+                         (DET_HEAD_NORM if norm else 0) | (DET_HEAD_ROTATE if rotate else 0))
+        self._keep = (x, out, gain)
+
+
+class AttnCache(C.Structure):
+    """det_attn_cache_t: one sequence's cached key and value rows."""
+
+    _fields_ = [("k_dev", C.c_void_p), ("v_dev", C.c_void_p), ("stride", C.c_uint64), ("rows", C.c_uint64),
+                ("first", C.c_uint64), ("wrap", C.c_uint64)]
+
+    def __init__(self, k=None, v=None, stride: int = 0, rows: int = 0, first: int = 0, wrap: int = 0):
+        super().__init__(_dev(k), _dev(v), stride, rows, first, wrap)
+        self._keep = (k, v)
+
+
+def attn_caches(caches) -> "C.Array":
+    """The views of a batch as the array Context.attention_tree takes (build it once, reuse it)."""
+    a = (AttnCache * len(caches))(*caches)
+    a._keep = list(caches)
+    return a
+
+
+def u32_array(values) -> "C.Array":
+    """Host words as the array Context.attention_tree takes for its drafted row counts."""
+    return (C.c_uint32 * len(values))(*values)
+
+
+def tree_masks(parents):
+    """det_tree_masks: (masks uint64, depths uint32) of drafted rows whose parents come before them (-1: none)."""
+    p = np.ascontiguousarray(parents, dtype=np.int32)
+    masks, depths = np.zeros(p.size, dtype=np.uint64), np.zeros(p.size, dtype=np.uint32)
+    st = lib().det_tree_masks(_ptr(p), p.size, _ptr(masks), _ptr(depths))
+    if st:
+        raise DetError(st, lib().det_ctx_last_error(None).decode())
+    return masks, depths
+
+
+class AdapterSpec(C.Structure):
+    """det_adapter_spec_t."""
+
+    _fields_ = [("rank", C.c_uint64), ("down_width", C.c_int32), ("down", C.c_void_p), ("down_scale", C.c_void_p),
+                ("up_width", C.c_int32), ("up", C.c_void_p), ("up_scale", C.c_void_p), ("scale", C.c_int32)]
+
+
+@dataclasses.dataclass
+class Adapter:
+    """One low-rank adapter: ``down`` [rank][cols], ``up`` [rows][rank] (int8 with a row scale, int16 or int32 Wgt
+    bits) and the Q16.16 ``scale`` of its product."""
+
+    down: np.ndarray
+    up: np.ndarray
+    scale: int = 65536
+    down_scale: Optional[np.ndarray] = None
+    up_scale: Optional[np.ndarray] = None
+
+
+class LogitRules(C.Structure):
+    """det_logit_rules_t: the decoding rules of Context.select_tokens (device arrays; None: no such rule).
+
+    ``penalties`` holds (repetition, frequency, presence) Q16.16 words per row."""
+
+    _fields_ = [("penalties_dev", C.c_void_p), ("ids_dev", C.c_void_p), ("n_ids", C.c_uint64),
+                ("spans_dev", C.c_void_p), ("spans_per_row", C.c_uint64), ("bias_begin_dev", C.c_void_p),
+                ("bias_ids_dev", C.c_void_p), ("bias_values_dev", C.c_void_p), ("n_bias", C.c_uint64),
+                ("mask_dev", C.c_void_p), ("mask_stride", C.c_uint64)]
+
+    def __init__(self, penalties=None, ids=None, n_ids: int = 0, spans=None, spans_per_row: int = 1, bias_begin=None,
+                 bias_ids=None, bias_values=None, n_bias: int = 0, mask=None, mask_stride: int = 0):
+        super().__init__(_dev(penalties), _dev(ids), n_ids, _dev(spans), spans_per_row, _dev(bias_begin),
+                         _dev(bias_ids), _dev(bias_values), n_bias, _dev(mask), mask_stride)
+        self._keep = (penalties, ids, spans, bias_begin, bias_ids, bias_values, mask)
 
 
 DETOKENIZE_FN = C.CFUNCTYPE(C.c_int64, C.POINTER(C.c_uint32), C.c_uint64, C.c_void_p, C.c_size_t, C.c_void_p)
@@ -271,6 +373,16 @@ def lib() -> C.CDLL:
         "det_argmax_first": (C.c_int, [P, P, u64, C.POINTER(C.c_uint32)]),
         "det_argmax_first_noalloc": (C.c_int, [P, P, u64, P]),
         "det_elementwise": (C.c_int, [P, C.c_int, P, P, u64, C.c_int32]),
+        "det_rope_table_create": (C.c_int, [P, C.POINTER(RopeSpec), C.POINTER(P)]),
+        "det_rope_table_free": (None, [P]),
+        "det_head_norm_rope": (C.c_int, [P, P, P, u64, u64, C.c_int64, P, u64]),
+        "det_kv_view": (C.c_int, [P, C.POINTER(AttnCache)]),
+        "det_tree_masks": (C.c_int, [P, u64, P, P]),
+        "det_attention_tree": (C.c_int, [P, P, P, u64, P, u64, P, P, u64, P, P, u64, u64, u64, P, u64]),
+        "det_adapters_create": (C.c_int, [P, u64, u64, P, u64, C.POINTER(P)]),
+        "det_adapters_free": (None, [P]),
+        "det_linear_adapters": (C.c_int, [P, P, P, u64, P, P, P]),
+        "det_select_tokens": (C.c_int, [P, P, u64, u64, u64, P, P, u64, P]),
         "det_model_create": (C.c_int, [P, C.POINTER(TextConfig), C.POINTER(P)]),
         "det_model_set_tensor": (C.c_int, [P, C.c_char_p, u64, P, C.c_int, P, P]),
         "det_model_load_detwgt": (C.c_int, [P, P, C.c_size_t]),
@@ -371,8 +483,8 @@ class Context:
 
     def close(self) -> None:
         if getattr(self, "handle", None):
-            order = {"Graph": 0, "Session": 0, "KvCache": 0, "Scratch": 0, "Model": 1, "Matrix": 2, "DeviceBuffer": 3,
-                     "Event": 4}
+            order = {"Graph": 0, "Session": 0, "KvCache": 0, "Scratch": 0, "Model": 1, "Matrix": 2, "Adapters": 2,
+                     "RopeTable": 2, "DeviceBuffer": 3, "Event": 4}
             for child in sorted(list(getattr(self, "_children", ())), key=lambda c: order.get(type(c).__name__, 5)):
                 child._release()
             self.lib.det_ctx_destroy(self.handle)
@@ -467,6 +579,35 @@ class Context:
     def elementwise(self, op: int, x: "DeviceBuffer", y: "DeviceBuffer | None", n: int, scalar: int = 0) -> None:
         yp = C.c_void_p(y.ptr) if y is not None else None
         self.check(self.lib.det_elementwise(self.handle, op, C.c_void_p(x.ptr), yp, n, scalar))
+
+    # -- verifying drafted tokens ------------------------------------------------
+    def head_norm_rope(self, table: "RopeTable | None", positions, rows: int, head_dim: int, eps: int, sets) -> None:
+        """Head norms and rotation of up to four sets of head rows (HeadRows) in one pass."""
+        arr = (HeadRows * len(sets))(*sets)
+        self.check(self.lib.det_head_norm_rope(self.handle, table.handle if table is not None else None,
+                                               _dev(positions), rows, head_dim, eps, arr, len(sets)))
+
+    def attention_tree(self, caches, drafts, q, q_stride: int, k, v, kv_stride: int, masks, starts, num_heads: int,
+                       num_kv_heads: int, head_dim: int, out, out_stride: int) -> None:
+        """Attention of drafted rows over each sequence's cache (attn_caches) and the drafted rows of their masks;
+        ``drafts`` holds each sequence's drafted rows (u32_array), ``starts`` (or None) each row's first cached row."""
+        if len(caches) != len(drafts):
+            raise ValueError("one drafted row count per cache is required")
+        self.check(self.lib.det_attention_tree(self.handle, caches, drafts, len(drafts), _dev(q), q_stride, _dev(k),
+                                               _dev(v), kv_stride, _dev(masks), _dev(starts), num_heads, num_kv_heads,
+                                               head_dim, _dev(out), out_stride))
+
+    def det_linear_adapters(self, w: "Matrix", adapters: "Adapters", m: int, act, index, out) -> None:
+        """det_linear_slab of m rows, each with the adapter index[t] (DET_NO_ADAPTER: none)."""
+        self.check(self.lib.det_linear_adapters(self.handle, w.handle, adapters.handle, m, _dev(act), _dev(index),
+                                                _dev(out)))
+
+    def select_tokens(self, logits, n: int, vocab: int, stride: int, rules: "LogitRules | None", out, out_stride: int,
+                      tokens) -> None:
+        """Decoding rules on n rows of logits (to ``out``, or None) and the chosen tokens (to ``tokens``, or None)."""
+        self.check(self.lib.det_select_tokens(self.handle, _dev(logits), n, vocab, stride,
+                                              C.byref(rules) if rules is not None else None, _dev(out), out_stride,
+                                              _dev(tokens)))
 
 
 class DeviceBuffer:
@@ -583,6 +724,75 @@ class Matrix:
     def _release(self) -> None:
         if self.handle and self.ctx.handle:
             self.ctx.lib.det_matrix_free(self.handle)
+        self.handle = None
+
+    def __del__(self):
+        try:
+            self._release()
+        except Exception:
+            pass
+
+
+class RopeTable:
+    """det_rope_table_t: the frequencies of one rotation. Numbers in Q32.32 (``base``, ``factor``, ``low_turns``,
+    ``high_turns``) except the Q16.16 ``amplitude``."""
+
+    def __init__(self, ctx: Context, rotary_dim: int, freq_base_dim: int, base: int, layout: int = DET_ROPE_HALF,
+                 scaling: int = DET_ROPE_SCALE_NONE, factor: int = 1 << 32, low_turns: int = 0, high_turns: int = 0,
+                 original_positions: int = 0, amplitude: int = 65536):
+        self.ctx = ctx
+        spec = RopeSpec(rotary_dim, freq_base_dim, base, layout, scaling, factor, low_turns, high_turns,
+                        original_positions, amplitude)
+        h = C.c_void_p()
+        ctx.check(ctx.lib.det_rope_table_create(ctx.handle, C.byref(spec), C.byref(h)))
+        self.handle = h
+        ctx._adopt(self)
+
+    def _release(self) -> None:
+        if self.handle and self.ctx.handle:
+            self.ctx.lib.det_rope_table_free(self.handle)
+        self.handle = None
+
+    def __del__(self):
+        try:
+            self._release()
+        except Exception:
+            pass
+
+
+class Adapters:
+    """det_adapters_t: the low-rank adapters (a list of Adapter) of one rows x cols projection."""
+
+    def __init__(self, ctx: Context, rows: int, cols: int, adapters):
+        self.ctx = ctx
+        widths = {np.dtype(np.int8): 8, np.dtype(np.int16): 16, np.dtype(np.int32): 32}
+        specs, keep = (AdapterSpec * max(len(adapters), 1))(), []
+        for s, ad in zip(specs, adapters):
+            down, up = np.ascontiguousarray(ad.down), np.ascontiguousarray(ad.up)
+            rank = down.shape[0]
+            if down.shape != (rank, cols) or up.shape != (rows, rank):
+                raise ValueError(f"adapter shapes {down.shape} and {up.shape} do not fit a {rows} x {cols} projection")
+            s.rank, s.scale = rank, ad.scale
+            for name, w, rs, length in (("down", down, ad.down_scale, rank), ("up", up, ad.up_scale, rows)):
+                setattr(s, name + "_width", widths[w.dtype])
+                setattr(s, name, w.ctypes.data)
+                if w.dtype == np.int8:
+                    if rs is None:
+                        raise ValueError("int8 adapters need a row scale")
+                    rs = np.ascontiguousarray(rs, dtype=np.int32)
+                    if rs.shape != (length,):
+                        raise ValueError("an adapter's row scale has one value per row")
+                    setattr(s, name + "_scale", rs.ctypes.data)
+                keep += [w, rs]
+        h = C.c_void_p()
+        ctx.check(ctx.lib.det_adapters_create(ctx.handle, rows, cols, specs, len(adapters), C.byref(h)))
+        self.handle = h
+        self.rows, self.cols, self.count = rows, cols, len(adapters)
+        ctx._adopt(self)
+
+    def _release(self) -> None:
+        if self.handle and self.ctx.handle:
+            self.ctx.lib.det_adapters_free(self.handle)
         self.handle = None
 
     def __del__(self):
@@ -836,6 +1046,13 @@ class KvCache:
         h = C.c_void_p()
         self.ctx.check(self.ctx.lib.det_kv_clone(self.handle, C.byref(h)))
         return KvCache(self.model, self.layer, 0, _handle=h)
+
+    def view(self) -> AttnCache:
+        """The cache's rows for Context.attention_tree (valid until it takes more tokens)."""
+        out = AttnCache()
+        self.ctx.check(self.ctx.lib.det_kv_view(self.handle, C.byref(out)))
+        out._keep = self
+        return out
 
     def _release(self) -> None:
         if self.handle and self.ctx.handle:
