@@ -253,7 +253,7 @@ int det_attention_tree(det_ctx_t* ctx, const det_attn_cache_t* caches, const uin
  * scale_act(B (A x), scale) to the projection's row, A = down [rank][cols] and
  * B = up [rows][rank], stored as det_matrix_upload stores them (element width
  * 8 with a row scale, 16 or 32; both products requantized as det_linear's).
- * rank 1 .. 256. */
+ * rank 1 .. 256, at most 4096 adapters. */
 typedef struct det_adapter_spec {
   uint64_t rank;
   int32_t down_width;

@@ -3355,25 +3355,18 @@ std::vector<int64_t> rope_frequencies(const det_rope_spec_t& sp) {
 }
 
 // B's rows in the layout of det::DevAdapter, from the tile-major upload.
-DevRef pack_up(det_ctx* ctx, const DevMatrix& M, size_t* scale_at, size_t* sum_at) {
+DevRef pack_up(det_ctx* ctx, const DevMatrix& M, size_t* scale_at) {
   const HostDigits h = untile(ctx, M);
   const uint64_t tiles = (h.rows + 15) / 16, kg = (h.cols + 15) / 16, planes = uint64_t(h.planes);
-  const size_t q_bytes = round_up(tiles * planes * kg * 256, 256);
-  *scale_at = q_bytes;
-  *sum_at = q_bytes + tiles * 16 * 4;
-  std::vector<uint8_t> buf(q_bytes + 2 * tiles * 16 * 4, 0);
+  *scale_at = round_up(tiles * planes * kg * 256, 256);
+  std::vector<uint8_t> buf(*scale_at + tiles * 16 * 4, 0);
   int32_t* scale = reinterpret_cast<int32_t*>(buf.data() + *scale_at);
-  int32_t* sum = reinterpret_cast<int32_t*>(buf.data() + *sum_at);
   for (uint64_t r = 0; r < h.rows; ++r) {
     scale[r] = h.scale[r];
-    int64_t s = 0;
     for (uint64_t p = 0; p < planes; ++p)
-      for (uint64_t c = 0; c < h.cols; ++c) {
-        const int8_t d = h.d[(p * h.rows + r) * h.cols + c];
-        buf[(((r >> 4) * planes + p) * kg + c / 16) * 256 + (r & 15) * 16 + c % 16] = uint8_t(d);
-        s += int64_t(d) * (int64_t(1) << (8 * p));
-      }
-    sum[r] = int32_t(s);  // (within int32 by the row-mass bound)
+      for (uint64_t c = 0; c < h.cols; c += 16)
+        std::memcpy(&buf[(((r >> 4) * planes + p) * kg + c / 16) * 256 + (r & 15) * 16],
+                    &h.d[(p * h.rows + r) * h.cols + c], std::min<uint64_t>(16, h.cols - c));
   }
   return to_device(ctx, buf.data(), buf.size());
 }
@@ -3811,8 +3804,9 @@ int det_adapters_create(det_ctx_t* ctx, uint64_t rows, uint64_t cols, const det_
     if (ctx->capturing) bail("det_ctx capture: adapters cannot be created inside a capture");
     if (rows == 0 || cols == 0) bail("an empty projection has no adapters");
     if (cols > 130000) bail("adapters of more than 130000 columns are not supported");
-    if (rows > UINT32_MAX) bail("too many rows");
-    if (n == 0 || n > 65536 || !specs) bail("1 to 65536 adapters are required");
+    if (rows > (uint64_t(1) << 23)) bail("adapters of more than 8388608 rows are not supported");
+    if (n == 0 || n > det::kAdapterMost || !specs)
+      bail("1 to " + std::to_string(det::kAdapterMost) + " adapters are required");
     OnDevice on(ctx);
     raw = new det_adapters;
     raw->ctx = ctx;
@@ -3829,10 +3823,10 @@ int det_adapters_create(det_ctx_t* ctx, uint64_t rows, uint64_t cols, const det_
       raw->down.push_back(upload_matrix(ctx, sp.rank, cols, sp.down_width, sp.down, sp.down_scale));
       const DevMatrix& A = raw->down.back();
       DevMatrix B = upload_matrix(ctx, rows, sp.rank, sp.up_width, sp.up, sp.up_scale);
-      size_t scale_at = 0, sum_at = 0;
+      size_t scale_at = 0;
       DevRef up;
       try {
-        up = pack_up(ctx, B, &scale_at, &sum_at);
+        up = pack_up(ctx, B, &scale_at);
       } catch (...) {
         free_matrix(B);
         throw;
@@ -3842,9 +3836,9 @@ int det_adapters_create(det_ctx_t* ctx, uint64_t rows, uint64_t cols, const det_
       raw->up.push_back(up);
       const int8_t* p = static_cast<const int8_t*>(up.get());
       det::DevAdapter d{};
-      d.a = A.q, d.a_scale = A.scale, d.a_rowsum = A.rowsum, d.a_planes = uint32_t(A.planes);
+      d.a = A.q, d.a_scale = A.scale, d.a_planes = uint32_t(A.planes);
       d.b = p, d.b_scale = reinterpret_cast<const int32_t*>(p + scale_at);
-      d.b_rowsum = reinterpret_cast<const int32_t*>(p + sum_at), d.b_planes = b_planes;
+      d.b_planes = b_planes;
       d.rank = uint32_t(sp.rank), d.kg = uint32_t((sp.rank + 15) / 16), d.scale = sp.scale;
       table.push_back(d);
       raw->max_rank = std::max(raw->max_rank, d.kg * 16);

@@ -64,15 +64,14 @@ void launch_tree_attention(const TreeArgs& a, const TreeSeq* seqs, uint32_t n, v
 struct DevAdapter {
   const int8_t* a;
   const int32_t* a_scale;
-  const int32_t* a_rowsum;
   const int8_t* b;
   const int32_t* b_scale;
-  const int32_t* b_rowsum;
   uint32_t rank, kg;
   uint32_t a_planes, b_planes;
   int32_t scale;
 };
 constexpr uint32_t kAdapterMaxRank = 256;
+constexpr uint32_t kAdapterMost = 4096;  // adapters of one set
 struct AdapterArgs {
   const DevAdapter* set;
   uint32_t n;
