@@ -13,7 +13,9 @@ namespace det {
 
 namespace {
 
-constexpr uint32_t kSpan = 4096;  // tokens per workgroup
+constexpr uint32_t kQuads = 4;               // groups of four tokens per thread
+constexpr uint32_t kSpan = 256 * 4 * kQuads;  // tokens per workgroup
+constexpr uint32_t kBatch = 8;                // history ids of a thread in flight
 
 // A row's choice so far: value (offset to unsigned) over the inverted index,
 // so that the larger key is the larger value, then the lower index; 0: none.
@@ -24,55 +26,175 @@ struct OpMaxU64 {
   __device__ __forceinline__ uint64_t operator()(uint64_t p, uint64_t q) const { return p > q ? p : q; }
 };
 
+// The history of a row as one list: its spans one after the other.
+struct History {
+  uint64_t at[8], len[8];
+  uint32_t n;
+  uint64_t total;
+};
+__device__ inline History history_of(const SelectArgs& a, uint64_t r) {
+  History h;
+  h.n = a.spans_per_row;
+  h.total = 0;
+#pragma unroll
+  for (uint32_t s = 0; s < 8; ++s) {
+    h.at[s] = h.len[s] = 0;
+    if (s < h.n) {
+      const uint64_t lo = a.spans[(r * h.n + s) * 2], e = a.spans[(r * h.n + s) * 2 + 1], hi = e < a.n_ids ? e : a.n_ids;
+      h.at[s] = lo;
+      h.len[s] = hi > lo ? hi - lo : 0;
+      h.total += h.len[s];
+    }
+  }
+  return h;
+}
+
+// One workgroup per row and 4096 tokens, sixteen tokens per thread, whose
+// logits and mask bits are loaded before the rules are looked at. A token that
+// a rule names has its bit in `named` (history: `seen`) and its sum in `sum`:
+// minus its penalties, plus its biases; only those entries are ever written or
+// read. Bound by the logits' bytes.
+template <bool VEC>
 __global__ __launch_bounds__(256) void k_select(SelectArgs a, uint64_t* keys, uint32_t parts) {
-  __shared__ uint32_t count[kSpan];
-  __shared__ unsigned long long bias[kSpan];
+  __shared__ unsigned long long sum[kSpan];
+  __shared__ uint32_t seen[kSpan / 32], named[kSpan / 32];
   __shared__ uint64_t red[4];
   const uint32_t tid = threadIdx.x, part = blockIdx.x;
   const uint64_t r = blockIdx.y, base = uint64_t(part) * kSpan;
   const uint32_t span = uint32_t(a.vocab - base < kSpan ? a.vocab - base : kSpan);
-  for (uint32_t i = tid; i < kSpan; i += 256) count[i] = 0, bias[i] = 0;
-  __syncthreads();
-  if (a.penalties && a.spans && a.ids)
-    for (uint32_t s = 0; s < a.spans_per_row; ++s) {
-      const uint64_t lo = a.spans[(r * a.spans_per_row + s) * 2], e = a.spans[(r * a.spans_per_row + s) * 2 + 1];
-      const uint64_t hi = e < a.n_ids ? e : a.n_ids;
-      for (uint64_t i = lo + tid; i < hi; i += 256) {
-        const uint64_t id = a.ids[i];
-        if (id >= base && id - base < span) atomicAdd(&count[id - base], 1u);
+  const int32_t* src = a.logits + r * a.ld + base;
+  int32_t x[kQuads][4];
+  uint32_t bits[kQuads];
+#pragma unroll
+  for (uint32_t q = 0; q < kQuads; ++q) {
+    const uint32_t t = 4 * (tid + 256 * q);
+    if (VEC && t + 4 <= span) {
+      const int4 v = *reinterpret_cast<const int4*>(src + t);
+      x[q][0] = v.x, x[q][1] = v.y, x[q][2] = v.z, x[q][3] = v.w;
+    } else {
+#pragma unroll
+      for (uint32_t e = 0; e < 4; ++e) x[q][e] = t + e < span ? src[t + e] : 0;
+    }
+    bits[q] = a.mask && t < span ? a.mask[r * a.mask_ld + (base + t) / 32] >> (t % 32) : 15u;
+    if (t + 4 > span) bits[q] &= t < span ? (1u << (span - t)) - 1 : 0u;
+  }
+  const bool penal = a.penalties && a.spans && a.ids, biased = a.bias_begin && a.bias_ids && a.bias_values;
+  SelectPenalty p{kOneAct, 0, 0};
+  if (penal || biased) {
+    for (uint32_t i = tid; i < kSpan / 32; i += 256) seen[i] = named[i] = 0;
+    History h{};
+    if (penal) {
+      p = a.penalties[r];
+      h = history_of(a, r);
+    }
+    // the batch of ids from `from` on: offsets into the part, kSpan for those of other parts
+    auto ids_of = [&](uint64_t from, uint32_t (&id)[kBatch]) {
+#pragma unroll
+      for (uint32_t b = 0; b < kBatch; ++b) {
+        uint64_t u = from + tid + 256 * b;
+        uint64_t at = 0;
+        bool on = false;
+#pragma unroll
+        for (uint32_t s = 0; s < 8; ++s) {
+          if (s >= h.n || on) continue;
+          if (u < h.len[s]) at = h.at[s] + u, on = true;
+          else u -= h.len[s];
+        }
+        id[b] = on ? a.ids[at] : 0xffffffffu;
+      }
+#pragma unroll
+      for (uint32_t b = 0; b < kBatch; ++b) {
+        const uint64_t o = uint64_t(id[b]) - base;
+        id[b] = o < span ? uint32_t(o) : kSpan;
+      }
+    };
+    uint64_t b0 = 0, b1 = 0;
+    if (biased) {
+      b0 = a.bias_begin[r];
+      b1 = a.bias_begin[r + 1];
+      b1 = b1 < a.n_bias ? b1 : a.n_bias;
+    }
+    uint32_t id[kBatch];
+    ids_of(0, id);  // (most histories are one batch, which is loaded once)
+    constexpr uint64_t kStep = 256 * kBatch;
+    __syncthreads();
+    // the named tokens' sums start at zero
+    for (uint64_t from = 0; from < h.total; from += kStep) {
+      if (from) ids_of(from, id);
+#pragma unroll
+      for (uint32_t b = 0; b < kBatch; ++b)
+        if (id[b] < kSpan) {
+          sum[id[b]] = 0;
+          atomicOr(&seen[id[b] / 32], 1u << (id[b] % 32));
+        }
+    }
+    for (uint64_t i = b0 + tid; i < b1; i += 256) {
+      const uint64_t o = uint64_t(a.bias_ids[i]) - base;
+      if (o < span) {
+        sum[o] = 0;
+        atomicOr(&named[o / 32], 1u << (o % 32));
       }
     }
-  if (a.bias_begin && a.bias_ids && a.bias_values) {
-    const uint64_t lo = a.bias_begin[r], e = a.bias_begin[r + 1], hi = e < a.n_bias ? e : a.n_bias;
-    for (uint64_t i = lo + tid; i < hi; i += 256) {
-      const uint64_t id = a.bias_ids[i];
-      if (id >= base && id - base < span)
-        atomicAdd(&bias[id - base], static_cast<unsigned long long>(int64_t(a.bias_values[i])));
+    __syncthreads();
+    for (uint64_t from = 0; from < h.total; from += kStep) {
+      if (h.total > kStep) ids_of(from, id);
+#pragma unroll
+      for (uint32_t b = 0; b < kBatch; ++b)
+        if (id[b] < kSpan) atomicAdd(&sum[id[b]], static_cast<unsigned long long>(-int64_t(p.frequency)));
+    }
+    for (uint64_t i = b0 + tid; i < b1; i += 256) {
+      const uint64_t o = uint64_t(a.bias_ids[i]) - base;
+      if (o < span) atomicAdd(&sum[o], static_cast<unsigned long long>(int64_t(a.bias_values[i])));
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t q = 0; q < kQuads; ++q) {
+      const uint32_t t = 4 * (tid + 256 * q), old = seen[t / 32] >> (t % 32), any = old | (named[t / 32] >> (t % 32));
+      if (!(any & 15u)) continue;
+#pragma unroll
+      for (uint32_t e = 0; e < 4; ++e) {
+        if (!((any >> e) & 1u)) continue;
+        int32_t v = x[q][e];
+        int64_t add = int64_t(sum[t + e]);
+        if ((old >> e) & 1u) {
+          if (p.repetition > 0 && p.repetition != kOneAct) v = v > 0 ? div_act(v, p.repetition) : mul_sat(v, p.repetition);
+          add -= p.presence;
+        }
+        x[q][e] = sat32(int64_t(v) + add);
+      }
     }
   }
-  __syncthreads();
-  SelectPenalty p{kOneAct, 0, 0};
-  if (a.penalties) p = a.penalties[r];
   uint64_t best = 0;
-  for (uint32_t i = tid; i < span; i += 256) {
-    const uint64_t token = base + i;
-    int32_t x = a.logits[r * a.ld + token];
-    const uint32_t c = count[i];
-    const int64_t b = int64_t(bias[i]);
-    if (c | (b != 0)) {
-      if (c && p.repetition > 0 && p.repetition != kOneAct) x = x > 0 ? div_act(x, p.repetition) : mul_sat(x, p.repetition);
-      x = sat32(int64_t(x) - int64_t(c) * p.frequency - (c ? p.presence : 0) + b);
+  int32_t* dst = a.out ? a.out + r * a.out_ld + base : nullptr;
+#pragma unroll
+  for (uint32_t q = 0; q < kQuads; ++q) {
+    const uint32_t t = 4 * (tid + 256 * q);
+    uint32_t at = 4;
+    int32_t top = INT32_MIN;
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) {
+      const bool ok = (bits[q] >> e) & 1u;
+      if (!ok) x[q][e] = INT32_MIN;
+      if (ok && (at == 4 || x[q][e] > top)) top = x[q][e], at = e;
     }
-    const bool ok = !a.mask || ((a.mask[r * a.mask_ld + token / 32] >> (token % 32)) & 1u);
-    if (!ok) x = INT32_MIN;
-    if (a.out) a.out[r * a.out_ld + token] = x;
-    const uint64_t k = ok ? choice_key(x, uint32_t(token)) : 0;
-    best = k > best ? k : best;
+    if (at < 4) {
+      const uint64_t k = choice_key(top, uint32_t(base) + t + at);
+      best = k > best ? k : best;
+    }
+    if (!dst) continue;
+    if (VEC && t + 4 <= span) {
+      *reinterpret_cast<int4*>(dst + t) = make_int4(x[q][0], x[q][1], x[q][2], x[q][3]);
+    } else {
+#pragma unroll
+      for (uint32_t e = 0; e < 4; ++e)
+        if (t + e < span) dst[t + e] = x[q][e];
+    }
   }
+  if (!keys) return;
   best = wave_reduce(best, OpMaxU64());
   if ((tid & 63) == 0) red[tid >> 6] = best;
   __syncthreads();
-  if (tid == 0 && keys) {
+  if (tid == 0) {
     for (int w = 1; w < 4; ++w) best = red[w] > best ? red[w] : best;
     keys[r * parts + part] = best;
   }
@@ -97,7 +219,10 @@ void launch_select(const SelectArgs& a, void* work, hipStream_t s) {
   if (a.n == 0 || (!a.tokens && !a.out)) return;
   const uint32_t parts = parts_of(a);
   uint64_t* keys = a.tokens ? static_cast<uint64_t*>(work) : nullptr;
-  hipLaunchKernelGGL(k_select, dim3(parts, unsigned(a.n)), dim3(256), 0, s, a, keys, parts);
+  auto aligned = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
+  const bool vec = a.ld % 4 == 0 && aligned(a.logits) && (!a.out || (a.out_ld % 4 == 0 && aligned(a.out)));
+  if (vec) hipLaunchKernelGGL(k_select<true>, dim3(parts, unsigned(a.n)), dim3(256), 0, s, a, keys, parts);
+  else hipLaunchKernelGGL(k_select<false>, dim3(parts, unsigned(a.n)), dim3(256), 0, s, a, keys, parts);
   if (a.tokens) hipLaunchKernelGGL(k_select_final, dim3(unsigned(a.n)), dim3(64), 0, s, keys, parts, a.tokens);
 }
 
