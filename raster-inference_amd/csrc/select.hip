@@ -26,29 +26,6 @@ struct OpMaxU64 {
   __device__ __forceinline__ uint64_t operator()(uint64_t p, uint64_t q) const { return p > q ? p : q; }
 };
 
-// The history of a row as one list: its spans one after the other.
-struct History {
-  uint64_t at[8], len[8];
-  uint32_t n;
-  uint64_t total;
-};
-__device__ inline History history_of(const SelectArgs& a, uint64_t r) {
-  History h;
-  h.n = a.spans_per_row;
-  h.total = 0;
-#pragma unroll
-  for (uint32_t s = 0; s < 8; ++s) {
-    h.at[s] = h.len[s] = 0;
-    if (s < h.n) {
-      const uint64_t lo = a.spans[(r * h.n + s) * 2], e = a.spans[(r * h.n + s) * 2 + 1], hi = e < a.n_ids ? e : a.n_ids;
-      h.at[s] = lo;
-      h.len[s] = hi > lo ? hi - lo : 0;
-      h.total += h.len[s];
-    }
-  }
-  return h;
-}
-
 // One workgroup per row and 4096 tokens, sixteen tokens per thread, whose
 // logits and mask bits are loaded before the rules are looked at. A token that
 // a rule names has its bit in `named` (history: `seen`) and its sum in `sum`:
@@ -62,6 +39,53 @@ __global__ __launch_bounds__(256) void k_select(SelectArgs a, uint64_t* keys, ui
   const uint32_t tid = threadIdx.x, part = blockIdx.x;
   const uint64_t r = blockIdx.y, base = uint64_t(part) * kSpan;
   const uint32_t span = uint32_t(a.vocab - base < kSpan ? a.vocab - base : kSpan);
+  // the rules' extents, then everything the workgroup reads in one go: its
+  // share of the history and the biases, its logits and mask bits
+  const bool penal = a.penalties && a.spans && a.ids, biased = a.bias_begin && a.bias_ids && a.bias_values;
+  const uint32_t* spans = a.spans + r * a.spans_per_row * 2;
+  const uint32_t n_ids = uint32_t(a.n_ids), n_bias = uint32_t(a.n_bias);  // (at most 2^28)
+  uint32_t total = 0, b0 = 0, b1 = 0;
+  SelectPenalty p{kOneAct, 0, 0};
+  if (penal) {
+    p = a.penalties[r];
+    for (uint32_t s = 0; s < a.spans_per_row; ++s) {
+      const uint32_t lo = spans[2 * s], hi = min(spans[2 * s + 1], n_ids);
+      total += hi > lo ? hi - lo : 0;
+    }
+  }
+  if (biased) {
+    b0 = a.bias_begin[r];
+    b1 = min(a.bias_begin[r + 1], n_bias);
+  }
+  // the batch of the row's history from entry `from` on (its spans one after the
+  // other): offsets into this part, kSpan for other parts' tokens
+  auto load_ids = [&](uint32_t from, uint32_t (&id)[kBatch]) {
+    uint32_t u[kBatch], at[kBatch];
+#pragma unroll
+    for (uint32_t b = 0; b < kBatch; ++b) u[b] = from + tid + 256 * b, at[b] = 0xffffffffu;
+    for (uint32_t s = 0; s < a.spans_per_row; ++s) {
+      const uint32_t lo = spans[2 * s], hi = min(spans[2 * s + 1], n_ids), len = hi > lo ? hi - lo : 0;
+#pragma unroll
+      for (uint32_t b = 0; b < kBatch; ++b) {
+        const bool in = u[b] < len;
+        if (in) at[b] = lo + u[b];
+        u[b] = in ? 0xffffffffu : u[b] - len;  // (stays above every length)
+      }
+    }
+#pragma unroll
+    for (uint32_t b = 0; b < kBatch; ++b) id[b] = at[b] < n_ids ? a.ids[at[b]] : 0xffffffffu;
+  };
+  auto offsets = [&](uint32_t (&id)[kBatch]) {
+#pragma unroll
+    for (uint32_t b = 0; b < kBatch; ++b) {
+      const uint32_t o = id[b] - uint32_t(base);  // (ids below the part wrap past it)
+      id[b] = o < span ? o : kSpan;
+    }
+  };
+  uint32_t id[kBatch], bias_id = 0xffffffffu;
+  int32_t bias_value = 0;
+  if (total) load_ids(0, id);
+  if (b0 + tid < b1) bias_id = a.bias_ids[b0 + tid], bias_value = a.bias_values[b0 + tid];
   const int32_t* src = a.logits + r * a.ld + base;
   int32_t x[kQuads][4];
   uint32_t bits[kQuads];
@@ -78,75 +102,38 @@ __global__ __launch_bounds__(256) void k_select(SelectArgs a, uint64_t* keys, ui
     bits[q] = a.mask && t < span ? a.mask[r * a.mask_ld + (base + t) / 32] >> (t % 32) : 15u;
     if (t + 4 > span) bits[q] &= t < span ? (1u << (span - t)) - 1 : 0u;
   }
-  const bool penal = a.penalties && a.spans && a.ids, biased = a.bias_begin && a.bias_ids && a.bias_values;
-  SelectPenalty p{kOneAct, 0, 0};
-  if (penal || biased) {
+  if (total || b0 < b1) {
     for (uint32_t i = tid; i < kSpan / 32; i += 256) seen[i] = named[i] = 0;
-    History h{};
-    if (penal) {
-      p = a.penalties[r];
-      h = history_of(a, r);
-    }
-    // the batch of ids from `from` on: offsets into the part, kSpan for those of other parts
-    auto ids_of = [&](uint64_t from, uint32_t (&id)[kBatch]) {
-#pragma unroll
-      for (uint32_t b = 0; b < kBatch; ++b) {
-        uint64_t u = from + tid + 256 * b;
-        uint64_t at = 0;
-        bool on = false;
-#pragma unroll
-        for (uint32_t s = 0; s < 8; ++s) {
-          if (s >= h.n || on) continue;
-          if (u < h.len[s]) at = h.at[s] + u, on = true;
-          else u -= h.len[s];
-        }
-        id[b] = on ? a.ids[at] : 0xffffffffu;
-      }
-#pragma unroll
-      for (uint32_t b = 0; b < kBatch; ++b) {
-        const uint64_t o = uint64_t(id[b]) - base;
-        id[b] = o < span ? uint32_t(o) : kSpan;
-      }
-    };
-    uint64_t b0 = 0, b1 = 0;
-    if (biased) {
-      b0 = a.bias_begin[r];
-      b1 = a.bias_begin[r + 1];
-      b1 = b1 < a.n_bias ? b1 : a.n_bias;
-    }
-    uint32_t id[kBatch];
-    ids_of(0, id);  // (most histories are one batch, which is loaded once)
-    constexpr uint64_t kStep = 256 * kBatch;
-    __syncthreads();
+    constexpr uint32_t kStep = 256 * kBatch;
+    if (total) offsets(id);
+    lds_barrier();
     // the named tokens' sums start at zero
-    for (uint64_t from = 0; from < h.total; from += kStep) {
-      if (from) ids_of(from, id);
+    auto name = [&](uint32_t o, uint32_t* set) {
+      sum[o] = 0;
+      atomicOr(&set[o / 32], 1u << (o % 32));
+    };
+    for (uint32_t from = 0; from < total; from += kStep) {
+      if (from) load_ids(from, id), offsets(id);
 #pragma unroll
       for (uint32_t b = 0; b < kBatch; ++b)
-        if (id[b] < kSpan) {
-          sum[id[b]] = 0;
-          atomicOr(&seen[id[b] / 32], 1u << (id[b] % 32));
-        }
+        if (id[b] < kSpan) name(id[b], seen);
     }
-    for (uint64_t i = b0 + tid; i < b1; i += 256) {
-      const uint64_t o = uint64_t(a.bias_ids[i]) - base;
-      if (o < span) {
-        sum[o] = 0;
-        atomicOr(&named[o / 32], 1u << (o % 32));
-      }
-    }
-    __syncthreads();
-    for (uint64_t from = 0; from < h.total; from += kStep) {
-      if (h.total > kStep) ids_of(from, id);
+    if (bias_id - uint32_t(base) < span) name(bias_id - uint32_t(base), named);
+    for (uint32_t i = b0 + 256 + tid; i < b1; i += 256)
+      if (a.bias_ids[i] - uint32_t(base) < span) name(a.bias_ids[i] - uint32_t(base), named);
+    lds_barrier();
+    const auto minus = static_cast<unsigned long long>(-int64_t(p.frequency));
+    for (uint32_t from = 0; from < total; from += kStep) {
+      if (total > kStep) load_ids(from, id), offsets(id);
 #pragma unroll
       for (uint32_t b = 0; b < kBatch; ++b)
-        if (id[b] < kSpan) atomicAdd(&sum[id[b]], static_cast<unsigned long long>(-int64_t(p.frequency)));
+        if (id[b] < kSpan) atomicAdd(&sum[id[b]], minus);
     }
-    for (uint64_t i = b0 + tid; i < b1; i += 256) {
-      const uint64_t o = uint64_t(a.bias_ids[i]) - base;
-      if (o < span) atomicAdd(&sum[o], static_cast<unsigned long long>(int64_t(a.bias_values[i])));
-    }
-    __syncthreads();
+    auto raise = [&](uint32_t o, int32_t v) { atomicAdd(&sum[o], static_cast<unsigned long long>(int64_t(v))); };
+    if (bias_id - uint32_t(base) < span) raise(bias_id - uint32_t(base), bias_value);
+    for (uint32_t i = b0 + 256 + tid; i < b1; i += 256)
+      if (a.bias_ids[i] - uint32_t(base) < span) raise(a.bias_ids[i] - uint32_t(base), a.bias_values[i]);
+    lds_barrier();
 #pragma unroll
     for (uint32_t q = 0; q < kQuads; ++q) {
       const uint32_t t = 4 * (tid + 256 * q), old = seen[t / 32] >> (t % 32), any = old | (named[t / 32] >> (t % 32));
