@@ -73,7 +73,9 @@ __global__ __launch_bounds__(256) void k_select(SelectArgs a, uint64_t* keys, ui
       }
     }
 #pragma unroll
-    for (uint32_t b = 0; b < kBatch; ++b) id[b] = at[b] < n_ids ? a.ids[at[b]] : 0xffffffffu;
+    for (uint32_t b = 0; b < kBatch; ++b) id[b] = a.ids[min(at[b], n_ids - 1)];  // (n_ids > 0 here)
+#pragma unroll
+    for (uint32_t b = 0; b < kBatch; ++b) id[b] = at[b] < n_ids ? id[b] : 0xffffffffu;
   };
   auto offsets = [&](uint32_t (&id)[kBatch]) {
 #pragma unroll
@@ -89,18 +91,24 @@ __global__ __launch_bounds__(256) void k_select(SelectArgs a, uint64_t* keys, ui
   const int32_t* src = a.logits + r * a.ld + base;
   int32_t x[kQuads][4];
   uint32_t bits[kQuads];
+  // (a wave's 256 tokens of one quad group are eight words of the mask: lane 8 q +
+  // w loads word w of group q, and each lane takes its four bits from there below)
+  uint32_t word = 0;
+  if (a.mask) {
+    const uint32_t l = tid & 63, t = 4 * (tid - l + 256 * (l / 8 % 4)) + 32 * (l % 8);
+    word = a.mask[r * a.mask_ld + (base + min(t, span - 1)) / 32];
+  }
+  if (VEC && span == kSpan) {  // (workgroup-uniform)
 #pragma unroll
-  for (uint32_t q = 0; q < kQuads; ++q) {
-    const uint32_t t = 4 * (tid + 256 * q);
-    if (VEC && t + 4 <= span) {
-      const int4 v = *reinterpret_cast<const int4*>(src + t);
+    for (uint32_t q = 0; q < kQuads; ++q) {
+      const int4 v = *reinterpret_cast<const int4*>(src + 4 * (tid + 256 * q));
       x[q][0] = v.x, x[q][1] = v.y, x[q][2] = v.z, x[q][3] = v.w;
-    } else {
-#pragma unroll
-      for (uint32_t e = 0; e < 4; ++e) x[q][e] = t + e < span ? src[t + e] : 0;
     }
-    bits[q] = a.mask && t < span ? a.mask[r * a.mask_ld + (base + t) / 32] >> (t % 32) : 15u;
-    if (t + 4 > span) bits[q] &= t < span ? (1u << (span - t)) - 1 : 0u;
+  } else {
+#pragma unroll
+    for (uint32_t q = 0; q < kQuads; ++q)
+#pragma unroll
+      for (uint32_t e = 0; e < 4; ++e) x[q][e] = src[min(4 * (tid + 256 * q) + e, span - 1)];
   }
   if (total || b0 < b1) {
     for (uint32_t i = tid; i < kSpan / 32; i += 256) seen[i] = named[i] = 0;
@@ -150,6 +158,12 @@ __global__ __launch_bounds__(256) void k_select(SelectArgs a, uint64_t* keys, ui
         x[q][e] = sat32(int64_t(v) + add);
       }
     }
+  }
+#pragma unroll
+  for (uint32_t q = 0; q < kQuads; ++q) {
+    const uint32_t t = 4 * (tid + 256 * q);
+    bits[q] = a.mask ? uint32_t(__shfl(int(word), int(8 * q + (tid & 63) / 8), 64)) >> (t % 32) : 15u;
+    if (t + 4 > span) bits[q] &= t < span ? (1u << (span - t)) - 1 : 0u;
   }
   uint64_t best = 0;
   int32_t* dst = a.out ? a.out + r * a.out_ld + base : nullptr;
