@@ -13,9 +13,10 @@ namespace det {
 
 namespace {
 
-constexpr uint32_t kQuads = 4;               // groups of four tokens per thread
-constexpr uint32_t kSpan = 256 * 4 * kQuads;  // tokens per workgroup
-constexpr uint32_t kBatch = 8;                // history ids of a thread in flight
+constexpr uint32_t kThreads = 512;
+constexpr uint32_t kQuads = 2;                     // groups of four tokens per thread
+constexpr uint32_t kSpan = kThreads * 4 * kQuads;  // tokens per workgroup
+constexpr uint32_t kBatch = 4;                // history ids of a thread in flight
 
 // A row's choice so far: value (offset to unsigned) over the inverted index,
 // so that the larger key is the larger value, then the lower index; 0: none.
@@ -26,16 +27,16 @@ struct OpMaxU64 {
   __device__ __forceinline__ uint64_t operator()(uint64_t p, uint64_t q) const { return p > q ? p : q; }
 };
 
-// One workgroup per row and 4096 tokens, sixteen tokens per thread, whose
+// One workgroup per row and 4096 tokens, eight tokens per thread, whose
 // logits and mask bits are loaded before the rules are looked at. A token that
 // a rule names has its bit in `named` (history: `seen`) and its sum in `sum`:
 // minus its penalties, plus its biases; only those entries are ever written or
 // read. Bound by the logits' bytes.
 template <bool VEC>
-__global__ __launch_bounds__(256) void k_select(SelectArgs a, uint64_t* keys, uint32_t parts) {
+__global__ __launch_bounds__(kThreads) void k_select(SelectArgs a, uint64_t* keys, uint32_t parts) {
   __shared__ unsigned long long sum[kSpan];
   __shared__ uint32_t seen[kSpan / 32], named[kSpan / 32];
-  __shared__ uint64_t red[4];
+  __shared__ uint64_t red[kThreads / 64];
   const uint32_t tid = threadIdx.x, part = blockIdx.x;
   const uint64_t r = blockIdx.y, base = uint64_t(part) * kSpan;
   const uint32_t span = uint32_t(a.vocab - base < kSpan ? a.vocab - base : kSpan);
@@ -62,7 +63,7 @@ __global__ __launch_bounds__(256) void k_select(SelectArgs a, uint64_t* keys, ui
   auto load_ids = [&](uint32_t from, uint32_t (&id)[kBatch]) {
     uint32_t u[kBatch], at[kBatch];
 #pragma unroll
-    for (uint32_t b = 0; b < kBatch; ++b) u[b] = from + tid + 256 * b, at[b] = 0xffffffffu;
+    for (uint32_t b = 0; b < kBatch; ++b) u[b] = from + tid + kThreads * b, at[b] = 0xffffffffu;
     for (uint32_t s = 0; s < a.spans_per_row; ++s) {
       const uint32_t lo = spans[2 * s], hi = min(spans[2 * s + 1], n_ids), len = hi > lo ? hi - lo : 0;
 #pragma unroll
@@ -95,24 +96,24 @@ __global__ __launch_bounds__(256) void k_select(SelectArgs a, uint64_t* keys, ui
   // w loads word w of group q, and each lane takes its four bits from there below)
   uint32_t word = 0;
   if (a.mask) {
-    const uint32_t l = tid & 63, t = 4 * (tid - l + 256 * (l / 8 % 4)) + 32 * (l % 8);
+    const uint32_t l = tid & 63, t = 4 * (tid - l + kThreads * (l / 8 % kQuads)) + 32 * (l % 8);
     word = a.mask[r * a.mask_ld + (base + min(t, span - 1)) / 32];
   }
   if (VEC && span == kSpan) {  // (workgroup-uniform)
 #pragma unroll
     for (uint32_t q = 0; q < kQuads; ++q) {
-      const int4 v = *reinterpret_cast<const int4*>(src + 4 * (tid + 256 * q));
+      const int4 v = *reinterpret_cast<const int4*>(src + 4 * (tid + kThreads * q));
       x[q][0] = v.x, x[q][1] = v.y, x[q][2] = v.z, x[q][3] = v.w;
     }
   } else {
 #pragma unroll
     for (uint32_t q = 0; q < kQuads; ++q)
 #pragma unroll
-      for (uint32_t e = 0; e < 4; ++e) x[q][e] = src[min(4 * (tid + 256 * q) + e, span - 1)];
+      for (uint32_t e = 0; e < 4; ++e) x[q][e] = src[min(4 * (tid + kThreads * q) + e, span - 1)];
   }
   if (total || b0 < b1) {
-    for (uint32_t i = tid; i < kSpan / 32; i += 256) seen[i] = named[i] = 0;
-    constexpr uint32_t kStep = 256 * kBatch;
+    for (uint32_t i = tid; i < kSpan / 32; i += kThreads) seen[i] = named[i] = 0;
+    constexpr uint32_t kStep = kThreads * kBatch;
     if (total) offsets(id);
     lds_barrier();
     // the named tokens' sums start at zero
@@ -127,7 +128,7 @@ __global__ __launch_bounds__(256) void k_select(SelectArgs a, uint64_t* keys, ui
         if (id[b] < kSpan) name(id[b], seen);
     }
     if (bias_id - uint32_t(base) < span) name(bias_id - uint32_t(base), named);
-    for (uint32_t i = b0 + 256 + tid; i < b1; i += 256)
+    for (uint32_t i = b0 + kThreads + tid; i < b1; i += kThreads)
       if (a.bias_ids[i] - uint32_t(base) < span) name(a.bias_ids[i] - uint32_t(base), named);
     lds_barrier();
     const auto minus = static_cast<unsigned long long>(-int64_t(p.frequency));
@@ -139,12 +140,12 @@ __global__ __launch_bounds__(256) void k_select(SelectArgs a, uint64_t* keys, ui
     }
     auto raise = [&](uint32_t o, int32_t v) { atomicAdd(&sum[o], static_cast<unsigned long long>(int64_t(v))); };
     if (bias_id - uint32_t(base) < span) raise(bias_id - uint32_t(base), bias_value);
-    for (uint32_t i = b0 + 256 + tid; i < b1; i += 256)
+    for (uint32_t i = b0 + kThreads + tid; i < b1; i += kThreads)
       if (a.bias_ids[i] - uint32_t(base) < span) raise(a.bias_ids[i] - uint32_t(base), a.bias_values[i]);
     lds_barrier();
 #pragma unroll
     for (uint32_t q = 0; q < kQuads; ++q) {
-      const uint32_t t = 4 * (tid + 256 * q), old = seen[t / 32] >> (t % 32), any = old | (named[t / 32] >> (t % 32));
+      const uint32_t t = 4 * (tid + kThreads * q), old = seen[t / 32] >> (t % 32), any = old | (named[t / 32] >> (t % 32));
       if (!(any & 15u)) continue;
 #pragma unroll
       for (uint32_t e = 0; e < 4; ++e) {
@@ -161,7 +162,7 @@ __global__ __launch_bounds__(256) void k_select(SelectArgs a, uint64_t* keys, ui
   }
 #pragma unroll
   for (uint32_t q = 0; q < kQuads; ++q) {
-    const uint32_t t = 4 * (tid + 256 * q);
+    const uint32_t t = 4 * (tid + kThreads * q);
     bits[q] = a.mask ? uint32_t(__shfl(int(word), int(8 * q + (tid & 63) / 8), 64)) >> (t % 32) : 15u;
     if (t + 4 > span) bits[q] &= t < span ? (1u << (span - t)) - 1 : 0u;
   }
@@ -169,7 +170,7 @@ __global__ __launch_bounds__(256) void k_select(SelectArgs a, uint64_t* keys, ui
   int32_t* dst = a.out ? a.out + r * a.out_ld + base : nullptr;
 #pragma unroll
   for (uint32_t q = 0; q < kQuads; ++q) {
-    const uint32_t t = 4 * (tid + 256 * q);
+    const uint32_t t = 4 * (tid + kThreads * q);
     uint32_t at = 4;
     int32_t top = INT32_MIN;
 #pragma unroll
@@ -196,7 +197,7 @@ __global__ __launch_bounds__(256) void k_select(SelectArgs a, uint64_t* keys, ui
   if ((tid & 63) == 0) red[tid >> 6] = best;
   __syncthreads();
   if (tid == 0) {
-    for (int w = 1; w < 4; ++w) best = red[w] > best ? red[w] : best;
+    for (int w = 1; w < int(kThreads / 64); ++w) best = red[w] > best ? red[w] : best;
     keys[r * parts + part] = best;
   }
 }
@@ -222,8 +223,8 @@ void launch_select(const SelectArgs& a, void* work, hipStream_t s) {
   uint64_t* keys = a.tokens ? static_cast<uint64_t*>(work) : nullptr;
   auto aligned = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
   const bool vec = a.ld % 4 == 0 && aligned(a.logits) && (!a.out || (a.out_ld % 4 == 0 && aligned(a.out)));
-  if (vec) hipLaunchKernelGGL(k_select<true>, dim3(parts, unsigned(a.n)), dim3(256), 0, s, a, keys, parts);
-  else hipLaunchKernelGGL(k_select<false>, dim3(parts, unsigned(a.n)), dim3(256), 0, s, a, keys, parts);
+  if (vec) hipLaunchKernelGGL(k_select<true>, dim3(parts, unsigned(a.n)), dim3(kThreads), 0, s, a, keys, parts);
+  else hipLaunchKernelGGL(k_select<false>, dim3(parts, unsigned(a.n)), dim3(kThreads), 0, s, a, keys, parts);
   if (a.tokens) hipLaunchKernelGGL(k_select_final, dim3(unsigned(a.n)), dim3(64), 0, s, keys, parts, a.tokens);
 }
 
