@@ -67,7 +67,7 @@ struct Launch {
   uint32_t n_seq, rows;  // row ids
   uint32_t chunk, chunks;    // keys per chunk of the scores and terms
   uint32_t wchunk, wchunks;  // of the weighted sums
-  uint32_t splits;           // key splits inside a weighted-sum block
+  uint32_t splits, groups;   // waves of a weighted-sum block: key splits x groups of 32 dims
   uint32_t row_blocks;
   uint32_t block_rows;
   int wide_k, wide_v;  // 16-byte aligned q and k rows, 8-byte aligned v rows
@@ -184,13 +184,26 @@ __device__ __forceinline__ void score_tile(const v4i (&k)[NSUB][3], const v4i* q
         acc[i + j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[s][j], b[s & 1][i], acc[i + j], 0, 0, 0);
     __builtin_amdgcn_sched_barrier(0);
   }
+  // dot = a0 + 2^8 a1 + .. + 2^32 a4, each sum below 2^25: carries of the low
+  // bytes leave floor(dot / 2^16) = v + 2^8 a3 + 2^16 a4 and a 16-bit remainder.
+  // Below 2^30 (any score under 4096.0) that is 32-bit arithmetic.
+  uint32_t far = 0;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    uint64_t dot = 0;
-#pragma unroll
-    for (int s = 0; s < 5; ++s) dot += uint64_t(int64_t(acc[s][r])) << (8 * s);
-    out[r] = requant(int64_t(dot));
+    const int32_t u = (acc[0][r] >> 8) + acc[1][r], v = (u >> 8) + acc[2][r];
+    const uint32_t rem = ((uint32_t(u) & 0xffu) << 8) | (uint32_t(acc[0][r]) & 0xffu);
+    far |= ((uint32_t(acc[4][r]) + 0x1000u) >> 13) | ((uint32_t(acc[3][r]) + 0x100000u) >> 21);
+    const uint32_t q = uint32_t(v) + (uint32_t(acc[3][r]) << 8) + (uint32_t(acc[4][r]) << 16);
+    out[r] = int32_t(q + uint32_t(rem + (q & 1u) > 0x8000u));
   }
+  if (__any(far != 0))
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      uint64_t dot = 0;
+#pragma unroll
+      for (int s = 0; s < 5; ++s) dot += uint64_t(int64_t(acc[s][r])) << (8 * s);
+      out[r] = requant(int64_t(dot));
+    }
 }
 
 // Scores: a block takes up to 64 query rows (digits in LDS, converted once) and
@@ -199,9 +212,9 @@ __device__ __forceinline__ void score_tile(const v4i (&k)[NSUB][3], const v4i* q
 template <int NSUB, int MODE>
 __global__ __launch_bounds__(kThreads, NSUB <= 4 ? 4 : 2) void k_tree_scores(Launch p) {
   extern __shared__ __attribute__((aligned(16))) int8_t lds[];  // [query tile][substep][digit][lane]
-  __shared__ int32_t wmax[kWaves][64];  // each wave's largest score of a row so far
+  __shared__ int32_t rmax[64];  // each row's largest score so far
   __shared__ Sight sight[64];
-  __shared__ uint32_t qwide;
+  __shared__ uint32_t qwide, last_start;
   const Item it = item_of(p, p.chunks);
   if (!it.on) return;
   const Seq& s = p.s[it.seq];
@@ -212,9 +225,13 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 ? 4 : 2) void k_tree_scores(Lau
   const uint32_t rows = min(R - r0, p.block_rows), tiles = (rows + 15) / 16;
   const uint32_t tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = l & 15, g = l >> 4;
   const uint32_t kvh = p.kv0 + it.kvh, hd = a.hd;
-  if (tid == 0) qwide = 0;
-  if (tid < 64) sight[tid] = sight_of(a, s, min(r0 + tid, R - 1) / a.groups);
-  for (uint32_t u = tid; u < kWaves * 64; u += kThreads) (&wmax[0][0])[u] = INT32_MIN;
+  if (tid < 64) {
+    const Sight v = sight_of(a, s, min(r0 + tid, R - 1) / a.groups);
+    const uint32_t m = uint32_t(wave_max64(int64_t(v.start)));
+    sight[tid] = v;
+    rmax[tid] = INT32_MIN;
+    if (tid == 0) qwide = 0, last_start = m;
+  }
   __syncthreads();
   for (uint32_t u = wave; u < tiles * NSUB; u += kWaves) {
     const uint32_t T = u / NSUB, sub = u % NSUB, row = min(r0 + 16 * T + i, R - 1);
@@ -244,19 +261,22 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 ? 4 : 2) void k_tree_scores(Lau
   const uint32_t id0 = s.id0 + it.kvh * R + r0;
   int32_t* sc = p.scores + s.score0 + uint64_t(it.kvh * R + r0) * s.score_ld;
   const uint64_t off = uint64_t(kvh) * hd;
+  const uint32_t seen_from = __builtin_amdgcn_readfirstlane(last_start);
   // scores of tile T and the keys from key0 on: stored, and the largest seen one kept
   auto finish = [&](uint32_t T, uint32_t key0, const int32_t (&out)[4]) {
     if (16 * T + i < rows)
       *reinterpret_cast<int4*>(sc + uint64_t(16 * T + i) * s.score_ld + key0 + 4 * g) =
           make_int4(out[0], out[1], out[2], out[3]);
-    const Sight v = sight[16 * T + i];
     int32_t m = INT32_MIN;
+    if (key0 >= seen_from && key0 + 16 <= s.rows) {  // (every row sees every key: wave-uniform)
+      m = max(max(out[0], out[1]), max(out[2], out[3]));
+    } else {
+      const Sight v = sight[16 * T + i];
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (sees(v, s.rows, key0 + 4 * g + r)) m = max(m, out[r]);
-    m = max(m, __shfl_xor(m, 16, 64));
-    m = max(m, __shfl_xor(m, 32, 64));
-    if (l < 16) wmax[wave][16 * T + l] = max(wmax[wave][16 * T + l], m);
+      for (int r = 0; r < 4; ++r)
+        if (sees(v, s.rows, key0 + 4 * g + r)) m = max(m, out[r]);
+    }
+    atomicMax(&rmax[16 * T + i], m);
   };
   uint64_t later0 = 0, later1 = 0;  // key tiles that are not narrow (at most 128 per wave and chunk; wave-uniform)
   for (uint32_t key0 = k0 + 16 * wave, t = 0; key0 < k1; key0 += 16 * kWaves, ++t) {
@@ -348,12 +368,7 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 ? 4 : 2) void k_tree_scores(Lau
   // leaves the lowest value, which changes no maximum; the terms look at what is
   // seen again)
   __syncthreads();
-  if (tid < rows) {
-    int32_t m = wmax[0][tid];
-#pragma unroll
-    for (uint32_t w = 1; w < kWaves; ++w) m = max(m, wmax[w][tid]);
-    p.pmax[uint64_t(id0 + tid) * p.chunks + it.chunk] = m;
-  }
+  if (tid < rows) p.pmax[uint64_t(id0 + tid) * p.chunks + it.chunk] = rmax[tid];
 }
 
 // Exp term (at most 2^32, and otherwise below 2^32 - 65000) in 32 bits.
@@ -430,12 +445,11 @@ __device__ inline Recip recip_of(int64_t sum) {
   }
   return r;
 }
-__device__ __forceinline__ uint32_t weight_of(uint32_t e, const Recip& r) {
-  const uint32_t half = 1u << (r.sh - 1), near = 1u << (r.sh - 13);
-  const uint32_t y = __umulhi(e, r.m) + half, f = y & (2 * half - 1);
-  uint32_t w = y >> r.sh;
-  if (f - near >= 2 * half - 2 * near) w = e ? uint32_t(softmax_weight(unpack_term(e), r.sum)) : 0;
-  return w;
+__device__ __forceinline__ uint32_t weight_of(uint32_t e, uint32_t m, uint32_t sh, bool& unsure) {
+  const uint32_t half = 1u << (sh - 1), near = 1u << (sh - 13);
+  const uint32_t y = __umulhi(e, m) + half, f = y & (2 * half - 1);
+  unsure = f - near >= 2 * half - 2 * near;
+  return y >> sh;
 }
 
 // Weighted sums: a block takes up to 16 RT query rows, one chunk of keys and
@@ -446,6 +460,8 @@ __device__ __forceinline__ uint32_t weight_of(uint32_t e, const Recip& r) {
 // key.
 // Weights above 32639 (at most two of a row) need a third digit; they go on
 // without 65536, which is added from the list of their keys.
+constexpr uint32_t wsum_rounds(int RT) { return RT == 4 ? 1 : 2; }
+constexpr uint32_t most_splits(int RT) { return wsum_rounds(RT) * kThreads / (RT * 128); }
 template <int RT>
 __global__ __launch_bounds__(kThreads, 2) void k_tree_wsum(Launch p) {
   extern __shared__ __attribute__((aligned(16))) int8_t lds[];  // [2][split][query tile][digit][lane]
@@ -462,7 +478,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_tree_wsum(Launch p) {
   if (r0 >= R || k0 >= k1) return;
   const uint32_t rows = min(R - r0, p.block_rows), id0 = s.id0 + it.kvh * R + r0;
   const uint32_t tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = l & 15, g = l >> 4;
-  const uint32_t kvh = p.kv0 + it.kvh, hd = a.hd, splits = p.splits, groups = kWaves / splits;
+  const uint32_t kvh = p.kv0 + it.kvh, hd = a.hd, splits = p.splits, groups = p.groups;
   const uint32_t split = wave / groups, dim0 = blockIdx.y * 256 + 32 * (wave % groups);
   const int32_t* terms = p.scores + s.score0 + uint64_t(it.kvh * R + r0) * s.score_ld;
   const uint32_t used = (n + p.chunk - 1) / p.chunk;
@@ -480,43 +496,82 @@ __global__ __launch_bounds__(kThreads, 2) void k_tree_wsum(Launch p) {
   }
   __syncthreads();
   const uint32_t per = 64 * splits;  // keys per step
-  // weights of step k (its first key) into the buffer: eight keys of a row at a time
-  auto put_weights = [&](uint32_t k, uint32_t buf) {
-    int8_t* dst = lds + buf * splits * RT * 2 * kOp;
-    for (uint32_t u = tid; u < splits * RT * 16 * 8; u += kThreads) {
-      const uint32_t r = u / 8 % (16 * RT), sp = u / (8 * 16 * RT), o = u % 8, key = k + 64 * sp + 8 * o;
-      uint32_t d[2][2] = {{0, 0}, {0, 0}};
+  // Weights of a step: eight keys of a row per thread and round, whose terms
+  // are loaded a step ahead.
+  constexpr uint32_t kRounds = wsum_rounds(RT);
+  const uint32_t items = splits * RT * 128;
+  auto load_terms = [&](uint32_t k, uint32_t u, uint32_t (&e)[8]) {
+    const uint32_t r = u / 8 % (16 * RT), key = k + 64 * (u / (128 * RT)) + 8 * (u % 8);
+    // (rows and keys past the end: any in range, not used)
+    const int4* src = reinterpret_cast<const int4*>(terms + uint64_t(min(r, rows - 1)) * s.score_ld + min(key, s.score_ld - 8));
+    const int4 t0 = src[0], t1 = src[1];
+    e[0] = uint32_t(t0.x), e[1] = uint32_t(t0.y), e[2] = uint32_t(t0.z), e[3] = uint32_t(t0.w);
+    e[4] = uint32_t(t1.x), e[5] = uint32_t(t1.y), e[6] = uint32_t(t1.z), e[7] = uint32_t(t1.w);
+  };
+  auto put_weights = [&](uint32_t k, uint32_t buf, uint32_t u, const uint32_t (&e)[8]) {
+    const uint32_t r = u / 8 % (16 * RT), sp = u / (128 * RT), o = u % 8, key = k + 64 * sp + 8 * o;
+    uint32_t w[8], d[2][2] = {{0, 0}, {0, 0}};
+    if (r < rows && key < k1) {
+      const uint32_t m = recip[r].m, sh = recip[r].sh;
+      uint32_t unsure = 0, most = 0;
       int32_t tot = 0;
-      if (r < rows && key < k1) {
-        const int4* src = reinterpret_cast<const int4*>(terms + uint64_t(r) * s.score_ld + key);
-        const int4 t0 = src[0], t1 = src[1];
-        const uint32_t e[8] = {uint32_t(t0.x), uint32_t(t0.y), uint32_t(t0.z), uint32_t(t0.w),
-                               uint32_t(t1.x), uint32_t(t1.y), uint32_t(t1.z), uint32_t(t1.w)};
-        const Recip rc = recip[r];
 #pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        bool no;
+        w[q] = weight_of(e[q], m, sh, no);
+        unsure |= uint32_t(no) << q;
+      }
+#pragma unroll 1
+      for (; unsure; unsure &= unsure - 1) {
+        const int at = __builtin_ctz(unsure);
+        uint32_t x = 0;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) x = q == at ? e[q] : x;
+        x = x ? uint32_t(softmax_weight(unpack_term(x), recip[r].sum)) : 0;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) w[q] = q == at ? x : w[q];
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        tot += int32_t(w[q]);
+        most = max(most, w[q]);
+      }
+      if (most > 32639)
+#pragma unroll 1
         for (int q = 0; q < 8; ++q) {
-          const uint32_t w = weight_of(e[q], rc);
-          tot += int32_t(w);
-          if (w > 32639) {
+          uint32_t x = 0;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) x = q == c ? w[c] : x;
+          if (x > 32639) {
             const uint32_t at = atomicAdd(&big_n[r], 1u);
             if (at < 2) big_key[r][at] = key + q;
           }
-          const uint32_t z = (w + 0x8080u) ^ 0x8080u;
-          d[0][q / 4] |= (z & 0xffu) << (8 * (q % 4));
-          d[1][q / 4] |= ((z >> 8) & 0xffu) << (8 * (q % 4));
         }
-        if (tot && blockIdx.y == 0) atomicAdd(&total[r], tot);
+      if (tot) {
+        if (blockIdx.y == 0) atomicAdd(&total[r], tot);
+        // digits of four weights at a time: bytes 0 and 1 of (w + 0x8080) ^ 0x8080
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t z[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) z[q] = w[4 * h + q] + 0x8080u;
+          const uint32_t a = __builtin_amdgcn_perm(z[1], z[0], 0x05010400u), b = __builtin_amdgcn_perm(z[3], z[2], 0x05010400u);
+          d[0][h] = __builtin_amdgcn_perm(b, a, 0x05040100u) ^ 0x80808080u;
+          d[1][h] = __builtin_amdgcn_perm(b, a, 0x07060302u) ^ 0x80808080u;
+        }
       }
-      // lane 16 (o / 2) + r % 16, bytes 8 (o % 2) ..
-      int8_t* at = dst + ((sp * RT + r / 16) * 2) * kOp + (16 * (o / 2) + r % 16) * 16 + 8 * (o % 2);
-      *reinterpret_cast<uint2*>(at) = make_uint2(d[0][0], d[0][1]);
-      *reinterpret_cast<uint2*>(at + kOp) = make_uint2(d[1][0], d[1][1]);
     }
+    // lane 16 (o / 2) + r % 16, bytes 8 (o % 2) ..
+    int8_t* at = lds + (buf * splits * RT + sp * RT + r / 16) * 2 * kOp + (16 * (o / 2) + r % 16) * 16 + 8 * (o % 2);
+    *reinterpret_cast<uint2*>(at) = make_uint2(d[0][0], d[0][1]);
+    *reinterpret_cast<uint2*>(at + kOp) = make_uint2(d[1][0], d[1][1]);
   };
   const uint64_t off = uint64_t(kvh) * hd;
   const uint32_t dim = dim0 + 2 * i;
+  const bool dims_on = split < splits && dim0 < hd;  // (wave-uniform)
   const uint32_t dim_in = dim + 1 < hd ? dim : (hd > 1 ? hd - 2 : 0);  // (sums of dims past hd are dropped)
   auto load_v = [&](uint32_t k, int32_t (&x)[16][2]) {
+    if (!dims_on) return;
     const uint32_t kk = k + 64 * split;
     uint64_t at = s.first + kk;
     if (s.wrap && at >= s.wrap) at -= s.wrap;
@@ -551,7 +606,6 @@ __global__ __launch_bounds__(kThreads, 2) void k_tree_wsum(Launch p) {
       for (int q = 0; q < 4; ++q) d[q][j] = int(w[q]);
     }
   };
-  const bool dims_on = dim0 < hd;  // (wave-uniform)
   v4i acc[RT][2][4];
 #pragma unroll
   for (int T = 0; T < RT; ++T)
@@ -559,9 +613,22 @@ __global__ __launch_bounds__(kThreads, 2) void k_tree_wsum(Launch p) {
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int q = 0; q < 4; ++q) acc[T][c][q] = v4i{0, 0, 0, 0};
-  int32_t x[16][2];
+  int32_t x[16][2] = {};
+  uint32_t e[kRounds][8];
+  auto all_terms = [&](uint32_t k) {
+#pragma unroll
+    for (uint32_t c = 0; c < kRounds; ++c)
+      if (tid + kThreads * c < items) load_terms(k, tid + kThreads * c, e[c]);
+  };
+  auto all_weights = [&](uint32_t k, uint32_t buf) {
+#pragma unroll
+    for (uint32_t c = 0; c < kRounds; ++c)
+      if (tid + kThreads * c < items) put_weights(k, buf, tid + kThreads * c, e[c]);
+  };
+  all_terms(k0);
   load_v(k0, x);
-  put_weights(k0, 0);
+  all_weights(k0, 0);
+  if (k0 + per < k1) all_terms(k0 + per);
   __syncthreads();
   uint32_t all = 0, buf = 0;
   for (uint32_t k = k0; k < k1; k += per, buf ^= 1) {
@@ -570,7 +637,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_tree_wsum(Launch p) {
     digit_words(x, 1, d[1], all);
     if (k + per < k1) {
       load_v(k + per, x);
-      put_weights(k + per, buf ^ 1);
+      all_weights(k + per, buf ^ 1);
+      if (k + 2 * per < k1) all_terms(k + 2 * per);
     }
     if (dims_on) {
       const v4i* w = reinterpret_cast<const v4i*>(lds + (buf * splits + split) * RT * 2 * kOp);
@@ -587,9 +655,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_tree_wsum(Launch p) {
           __builtin_amdgcn_sched_barrier(0);
         }
     }
-    __syncthreads();
+    lds_barrier();  // (the next step's loads stay in flight)
   }
   if (all) vwide = 1;
+  __syncthreads();
   // lane l, component r: row 16 T + 4 g + r, dims dim and dim + 1
   const uint32_t plane = it.chunk * splits + split;
   int64_t* out = p.planes + (uint64_t(plane) * p.rows + id0) * hd;
@@ -637,7 +706,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_tree_wsum(Launch p) {
 #pragma unroll 1
   for (uint32_t k = k0; k < k1; k += per) {
     __syncthreads();
-    put_weights(k, 0);
+    all_terms(k);
+    all_weights(k, 0);
     load_v(k, x);
     __syncthreads();
     if (!dims_on) continue;
@@ -665,8 +735,9 @@ __global__ __launch_bounds__(kThreads, 2) void k_tree_wsum(Launch p) {
   put(std::integral_constant<int, 3>(), std::integral_constant<int, 3>(), true);
 }
 
-// Join: a wave per (row, 64 dims).
+// Join: a block per (row, 64 dims), its waves a share of the planes each.
 __global__ __launch_bounds__(256) void k_tree_join(Launch p) {
+  __shared__ uint64_t share[4][64];
   const uint32_t l = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t id = blockIdx.x;
   uint32_t b = 0;
@@ -695,12 +766,24 @@ __global__ __launch_bounds__(256) void k_tree_join(Launch p) {
     extra = int64_t(add_sat(w, sub_sat(kOneAct, sat32(tot)))) - w;
     v = row_ptr(s, s.v, a.v, a.kv_ld, first, uint64_t(kvh) * a.hd);
   }
-  for (uint32_t d = 64 * wave + l; d < a.hd; d += 256) {
-    uint64_t y = 0;
-    for (uint32_t q = 0; q < wused * p.splits; ++q) y += uint64_t(p.planes[(uint64_t(q) * p.rows + id) * a.hd + d]);
-    if (v) y += uint64_t(extra * v[d]);
-    out[d] = v ? requant(int64_t(y)) : 0;
+  const uint32_t d = 64 * blockIdx.y + l, in = min(d, a.hd - 1), planes = wused * p.splits;
+  const int64_t* src = p.planes + uint64_t(id) * a.hd + in;
+  const uint64_t ld = uint64_t(p.rows) * a.hd;
+  uint64_t y = 0;
+  uint32_t q = wave;
+  for (; q + 12 < planes; q += 16) {
+    uint64_t t[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) t[u] = uint64_t(src[(q + 4 * u) * ld]);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) y += t[u];
   }
+  for (; q < planes; q += 4) y += uint64_t(src[q * ld]);
+  share[wave][l] = y;
+  __syncthreads();
+  if (wave || d >= a.hd) return;
+  for (int w = 1; w < 4; ++w) y += share[w][l];
+  out[d] = v ? requant(int64_t(y + uint64_t(extra * to_global(v)[d]))) : 0;
 }
 
 uint64_t up(uint64_t v, uint64_t a) { return (v + a - 1) / a * a; }
@@ -771,14 +854,15 @@ uint64_t plan(const TreeArgs& a, const TreeSeq* seqs, const Group& g, Launch& p)
   }
   p.wide_k = w4;
   p.wide_v = w2;
-  // 64 query rows per block, 32 where their digits take more than half the LDS
-  p.block_rows = std::min<uint32_t>(uint32_t(up(most, 16)), a.hd <= 256 ? 64 : 32);
+  // 64 query rows per block; 32 where their digits would take more than half the
+  // LDS, or where the waves of a weighted-sum block share the keys instead of the dims
+  p.block_rows = std::min<uint32_t>(uint32_t(up(most, 16)), a.hd > 128 && a.hd <= 256 ? 64 : 32);
   p.row_blocks = (most + p.block_rows - 1) / p.block_rows;
   units = uint64_t(p.n_seq) * g.nkv * p.row_blocks;
   p.chunk = chunk_of(keys, units, 1024, 16 * kWaves);
   p.chunks = uint32_t((keys + p.chunk - 1) / p.chunk);
-  const uint32_t groups = a.hd <= 32 ? 1 : a.hd <= 64 ? 2 : a.hd <= 128 ? 4 : 8;
-  p.splits = kWaves / groups;
+  p.groups = a.hd <= 32 ? 1 : a.hd <= 64 ? 2 : a.hd <= 128 ? 4 : 8;
+  p.splits = std::min(kWaves / p.groups, most_splits(p.block_rows <= 16 ? 1 : p.block_rows <= 32 ? 2 : 4));
   p.wchunk = chunk_of(keys, units * ((a.hd + kMaxDimsBlock - 1) / kMaxDimsBlock), 512, std::max(128u, 64 * p.splits));
   p.wchunks = uint32_t((keys + p.wchunk - 1) / p.wchunk);
   uint64_t at = 0;
@@ -847,7 +931,7 @@ void launch_tree_attention(const TreeArgs& a, const TreeSeq* seqs, uint32_t n, v
     if (p.block_rows <= 16) launch_wsum<1>(p, blocks(p.wchunks), s);
     else if (p.block_rows <= 32) launch_wsum<2>(p, blocks(p.wchunks), s);
     else launch_wsum<4>(p, blocks(p.wchunks), s);
-    hipLaunchKernelGGL(k_tree_join, dim3(p.rows), dim3(256), 0, s, p);
+    hipLaunchKernelGGL(k_tree_join, dim3(p.rows, (a.hd + 63) / 64), dim3(256), 0, s, p);
   });
 }
 
