@@ -331,6 +331,34 @@ DET_HD int64_t softmax_exp(int32_t logit, int32_t max_logit) {
   return rshift_rte(t, unsigned(shift));  // shift <= 23 here
 }
 
+// softmax_exp(logit, max_logit) of a gap d = max_logit - logit below 2^20, as
+// the double that it is exactly (a whole number of at most 2^32), in about 35
+// instructions against 140: d 2^16 / ln2 and its remainder from one high
+// product; the powers' rounded products from multiply-adds with half a unit (a
+// tie leaves a zero low word: softmax_exp itself then decides); the quotients by
+// 2, 6, 24 and 120 as rounded products with the divisors' reciprocals, the sum
+// and its shift in double arithmetic, whose rounding is half to even. That
+// every quotient has the exact rounding, ties among them, was checked for every
+// value the powers take; the sums are whole numbers below 2^34.
+// k_tree_terms at 4096 rows of 8256 keys: 126 -> 61 us.
+DET_HD double softmax_term(uint32_t d) {
+  const uint32_t shift = uint32_t((uint64_t(d << 12) * 3098164009u) >> 32) >> 27;
+  const uint32_t r1 = (d << 16) - shift * 2977044472u;
+  const uint64_t half = 0x80000000u;
+  const uint64_t p2 = uint64_t(r1) * r1 + half;
+  const uint32_t r2 = uint32_t(p2 >> 32);
+  const uint64_t p3 = uint64_t(r2) * r1 + half;
+  const uint32_t r3 = uint32_t(p3 >> 32);
+  const uint64_t p4 = uint64_t(r3) * r1 + half;
+  const uint32_t r4 = uint32_t(p4 >> 32);
+  const uint64_t p5 = uint64_t(r4) * r1 + half;
+  const uint32_t r5 = uint32_t(p5 >> 32);
+  if (!uint32_t(p2) | !uint32_t(p3) | !uint32_t(p4) | !uint32_t(p5)) return double(softmax_exp(0, int32_t(d)));
+  const double t = (4294967296.0 - double(r1)) + (__builtin_rint(double(r2) * 0.5) - __builtin_rint(double(r3) * (1.0 / 6))) +
+                   (__builtin_rint(double(r4) * (1.0 / 24)) - __builtin_rint(double(r5) * (1.0 / 120)));
+  return __builtin_rint(__builtin_ldexp(t, -int(shift)));
+}
+
 // Softmax raw weight: requantize(div_acc(exp, sum)) (ops.rs:266-268) for the
 // softmax domain 0 <= exp <= min(sum, 2^32), sum > 0: round(exp * 2^32 / sum)
 // ties to even, then requantize. A double estimate is within one of the floor

@@ -176,7 +176,7 @@ __device__ __forceinline__ void score_tile(const v4i (&k)[NSUB][3], const v4i* q
   for (int s = 0; s < NSUB; ++s) {
     if (s + 1 < NSUB)
 #pragma unroll
-      for (int i = 0; i < 3; ++i) b[(s + 1) & 1][i] = q[((s + 1) * 5 + i) * 64 + l];
+      for (int i = 0; i < 3; ++i) b[(s + 1) & 1][i] = q[((s + 1) * 3 + i) * 64 + l];
 #pragma unroll
     for (int i = 0; i < 3; ++i)
 #pragma unroll
@@ -233,27 +233,33 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 ? 4 : 2) void k_tree_scores(Lau
     if (tid == 0) qwide = 0, last_start = m;
   }
   __syncthreads();
+  // this lane's row of query tile T, and its values [dim, dim + 4)
+  auto q_row = [&](uint32_t T) {
+    const uint32_t row = min(r0 + 16 * T + i, R - 1);
+    return a.q + (s.row0 + row / a.groups) * a.q_ld + uint64_t(kvh * a.groups + row % a.groups) * hd;
+  };
+  auto load_q = [&](const int32_t* src, uint32_t dim, int32_t (&x)[4]) {
+    load4<MODE>(src, dim, hd, x);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (dim + e >= hd) x[e] = 0;
+  };
   for (uint32_t u = wave; u < tiles * NSUB; u += kWaves) {
-    const uint32_t T = u / NSUB, sub = u % NSUB, row = min(r0 + 16 * T + i, R - 1);
-    const int32_t* src = a.q + (s.row0 + row / a.groups) * a.q_ld + uint64_t(kvh * a.groups + row % a.groups) * hd;
-    uint32_t d[5][4], all = 0;
+    const uint32_t sub = u % NSUB;
+    const int32_t* src = q_row(u / NSUB);
+    uint32_t d[3][4], all = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint32_t dim = 64 * sub + 16 * j + 4 * g;
       int32_t x[4];
-      load4<MODE>(src, dim, hd, x);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (dim + e >= hd) x[e] = 0;
+      load_q(src, 64 * sub + 16 * j + 4 * g, x);
       uint32_t w[4];
       digits4(x, w, all);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) d[q][j] = w[q];
-      d[4][j] = top4(x);
+      for (int q = 0; q < 3; ++q) d[q][j] = w[q];
     }
-    v4i* dst = reinterpret_cast<v4i*>(lds) + uint64_t(u) * 5 * 64 + l;
+    v4i* dst = reinterpret_cast<v4i*>(lds) + uint64_t(u) * 3 * 64 + l;
 #pragma unroll
-    for (int q = 0; q < 5; ++q) dst[q * 64] = v4i{int(d[q][0]), int(d[q][1]), int(d[q][2]), int(d[q][3])};
+    for (int q = 0; q < 3; ++q) dst[q * 64] = v4i{int(d[q][0]), int(d[q][1]), int(d[q][2]), int(d[q][3])};
     if (__any(all != 0) && l == 0) qwide = 1;
   }
   __syncthreads();
@@ -317,7 +323,7 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 ? 4 : 2) void k_tree_scores(Lau
 #pragma unroll 1
     for (uint32_t T = 0; T < tiles; ++T) {
       int32_t out[4];
-      score_tile<NSUB>(k3, reinterpret_cast<const v4i*>(lds) + uint64_t(T) * NSUB * 5 * 64, l, out);
+      score_tile<NSUB>(k3, reinterpret_cast<const v4i*>(lds) + uint64_t(T) * NSUB * 3 * 64, l, out);
       finish(T, key0, out);
     }
   }
@@ -331,20 +337,25 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 ? 4 : 2) void k_tree_scores(Lau
       const int32_t* src = row_ptr(s, s.k, a.k, a.kv_ld, key0 + i, off);
 #pragma unroll 1
       for (uint32_t T = 0; T < tiles; ++T) {
-        const v4i* q = reinterpret_cast<const v4i*>(lds) + uint64_t(T) * NSUB * 5 * 64;
+        const int32_t* qsrc = q_row(T);
         uint64_t dot[4] = {0, 0, 0, 0};
 #pragma unroll 1
         for (uint32_t sub = 0; sub < nsub; ++sub) {
-          v4i k5[5];
+          v4i k5[5], q5[5];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             int32_t y[4];
-            load4<MODE>(src, 64 * sub + 16 * j + 4 * g, hd, y);
             uint32_t w[4], unused = 0;
+            load4<MODE>(src, 64 * sub + 16 * j + 4 * g, hd, y);
             digits4(y, w, unused);
 #pragma unroll
             for (int c = 0; c < 4; ++c) k5[c][j] = int(w[c]);
             k5[4][j] = int(top4(y));
+            load_q(qsrc, 64 * sub + 16 * j + 4 * g, y);
+            digits4(y, w, unused);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) q5[c][j] = int(w[c]);
+            q5[4][j] = int(top4(y));
           }
 #pragma unroll
           for (int c = 0; c < 8; ++c) {  // (digits 4 times 4 are past 2^64)
@@ -352,7 +363,7 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 ? 4 : 2) void k_tree_scores(Lau
 #pragma unroll
             for (int j = 0; j < 5; ++j)
               if (c - j >= 0 && c - j < 5)
-                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(k5[j], q[(sub * 5 + c - j) * 64 + l], acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(k5[j], q5[c - j], acc, 0, 0, 0);
 #pragma unroll
             for (int r = 0; r < 4; ++r) dot[r] += uint64_t(int64_t(acc[r])) << (8 * c);
             __builtin_amdgcn_sched_barrier(0);
@@ -371,8 +382,7 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 ? 4 : 2) void k_tree_scores(Lau
   if (tid < rows) p.pmax[uint64_t(id0 + tid) * p.chunks + it.chunk] = rmax[tid];
 }
 
-// Exp term (at most 2^32, and otherwise below 2^32 - 65000) in 32 bits.
-__device__ inline uint32_t pack_term(int64_t v) { return v >> 32 ? 0xffffffffu : uint32_t(v); }
+// An exp term (at most 2^32, and otherwise below 2^32 - 65000) from its 32 bits.
 __device__ inline int64_t unpack_term(uint32_t e) { return int64_t(uint64_t(e) + (e == 0xffffffffu)); }
 
 // Terms: one wave per (row, chunk).
@@ -391,33 +401,34 @@ __global__ __launch_bounds__(256) void k_tree_terms(Launch p) {
   m = int32_t(wave_max64(m));
   const Sight v = sight_of(p.a, s, local % R / p.a.groups);
   int32_t* sc = p.scores + s.score0 + uint64_t(local) * s.score_ld;
-  int64_t sum = 0;
+  double sum = 0;  // (whole numbers below 2^53: exact in any order)
   uint32_t first = 0xffffffffu;
   const uint32_t k2 = min((k1 + 63) & ~63u, s.score_ld);  // (whole substeps of the weighted sums)
+  const bool plain = v.start <= k0 && k1 <= s.rows;       // the row sees the whole chunk
   for (uint32_t kb = k0; kb < k2; kb += 256) {
     int32_t x[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const uint32_t k = kb + 64 * u + l;
-      x[u] = k < k1 ? sc[k] : 0;
-    }
+    for (int u = 0; u < 4; ++u) x[u] = sc[min(kb + 64 * u + l, k2 - 1)];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const uint32_t k = kb + 64 * u + l;
-      const bool seen = k < k1 && sees(v, s.rows, k);
-      int64_t e = 0;
-      if (__any(seen && uint32_t(m) - uint32_t(x[u]) < (1u << 20)) && seen) {
-        e = softmax_exp(x[u], m);
-        if (x[u] == m) first = min(first, k);
+      const uint32_t k = kb + 64 * u + l, gap = uint32_t(m) - uint32_t(x[u]);
+      bool in = k < k1 && gap < (1u << 20);
+      if (!plain) in = in && sees(v, s.rows, k);
+      double e = 0;
+      if (__any(in)) {
+        e = in ? softmax_term(gap) : 0.0;
+        if (in && gap == 0) first = min(first, k);
+        sum += e;
       }
-      sum += e;
-      if (k < k2) sc[k] = int32_t(pack_term(e));
+      // (2^32 in 32 bits: all ones, which no other term is)
+      if (k < k2) sc[k] = int32_t(uint32_t(__builtin_fmin(e, 4294967295.0)));
     }
   }
-  sum = wave_sum_wrap64(sum);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
   first = ~uint32_t(wave_max64(int64_t(~first)));
   if (l == 0) {
-    p.psum[uint64_t(id) * p.chunks + chunk] = sum;
+    p.psum[uint64_t(id) * p.chunks + chunk] = int64_t(sum);
     p.pfirst[uint64_t(id) * p.chunks + chunk] = first;
   }
 }
@@ -735,9 +746,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_tree_wsum(Launch p) {
   put(std::integral_constant<int, 3>(), std::integral_constant<int, 3>(), true);
 }
 
-// Join: a block per (row, 64 dims), its waves a share of the planes each.
+// Join: a wave per (row, 64 dims), or four with a share of the planes each where
+// there are many.
+template <int SHARES>
 __global__ __launch_bounds__(256) void k_tree_join(Launch p) {
-  __shared__ uint64_t share[4][64];
   const uint32_t l = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t id = blockIdx.x;
   uint32_t b = 0;
@@ -766,24 +778,28 @@ __global__ __launch_bounds__(256) void k_tree_join(Launch p) {
     extra = int64_t(add_sat(w, sub_sat(kOneAct, sat32(tot)))) - w;
     v = row_ptr(s, s.v, a.v, a.kv_ld, first, uint64_t(kvh) * a.hd);
   }
-  const uint32_t d = 64 * blockIdx.y + l, in = min(d, a.hd - 1), planes = wused * p.splits;
+  const uint32_t d = 64 * (blockIdx.y * (4 / SHARES) + wave / SHARES) + l, in = min(d, a.hd - 1);
+  const uint32_t planes = wused * p.splits;
   const int64_t* src = p.planes + uint64_t(id) * a.hd + in;
   const uint64_t ld = uint64_t(p.rows) * a.hd;
   uint64_t y = 0;
-  uint32_t q = wave;
-  for (; q + 12 < planes; q += 16) {
+  uint32_t q = wave % SHARES;
+  for (; q + 3 * SHARES < planes; q += 4 * SHARES) {
     uint64_t t[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) t[u] = uint64_t(src[(q + 4 * u) * ld]);
+    for (int u = 0; u < 4; ++u) t[u] = uint64_t(src[(q + u * SHARES) * ld]);
 #pragma unroll
     for (int u = 0; u < 4; ++u) y += t[u];
   }
-  for (; q < planes; q += 4) y += uint64_t(src[q * ld]);
-  share[wave][l] = y;
-  __syncthreads();
-  if (wave || d >= a.hd) return;
-  for (int w = 1; w < 4; ++w) y += share[w][l];
-  out[d] = v ? requant(int64_t(y + uint64_t(extra * to_global(v)[d]))) : 0;
+  for (; q < planes; q += SHARES) y += uint64_t(src[q * ld]);
+  if constexpr (SHARES > 1) {
+    __shared__ uint64_t share[4][64];
+    share[wave][l] = y;
+    __syncthreads();
+    if (wave) return;
+    for (int w = 1; w < 4; ++w) y += share[w][l];
+  }
+  if (d < a.hd) out[d] = v ? requant(int64_t(y + uint64_t(extra * to_global(v)[d]))) : 0;
 }
 
 uint64_t up(uint64_t v, uint64_t a) { return (v + a - 1) / a * a; }
@@ -817,13 +833,12 @@ void for_groups(const TreeArgs& a, const TreeSeq* seqs, uint32_t n, F&& f) {
   }
 }
 
-// Chunks of at least `least` keys (doubled until the blocks of `units` row
-// blocks per chunk come below `want`): enough blocks to fill the device, and
-// no more partial results than that takes.
-uint32_t chunk_of(uint64_t keys, uint64_t units, uint64_t want, uint32_t least) {
-  uint32_t c = least;
-  while (c < 16384 && units * ((keys + c - 1) / c) > want) c *= 2;
-  return c;
+// Keys per chunk: equal shares of the longest sequence, so that `units` blocks
+// per chunk make `want` blocks, what the device runs at once (in whole granules;
+// at most 16384 keys, which bounds the int32 sums and a wave's key tiles).
+uint32_t chunk_of(uint64_t keys, uint64_t units, uint64_t want, uint32_t granule) {
+  const uint64_t n = std::max<uint64_t>(want / units, 1);
+  return uint32_t(std::min<uint64_t>(up((keys + n - 1) / n, granule), 16384 / granule * granule));
 }
 
 // The launch of a group without its scratch pointers; returns the scratch's bytes.
@@ -859,11 +874,11 @@ uint64_t plan(const TreeArgs& a, const TreeSeq* seqs, const Group& g, Launch& p)
   p.block_rows = std::min<uint32_t>(uint32_t(up(most, 16)), a.hd > 128 && a.hd <= 256 ? 64 : 32);
   p.row_blocks = (most + p.block_rows - 1) / p.block_rows;
   units = uint64_t(p.n_seq) * g.nkv * p.row_blocks;
-  p.chunk = chunk_of(keys, units, 1024, 16 * kWaves);
+  p.chunk = chunk_of(keys, units, 512, 16 * kWaves);
   p.chunks = uint32_t((keys + p.chunk - 1) / p.chunk);
   p.groups = a.hd <= 32 ? 1 : a.hd <= 64 ? 2 : a.hd <= 128 ? 4 : 8;
   p.splits = std::min(kWaves / p.groups, most_splits(p.block_rows <= 16 ? 1 : p.block_rows <= 32 ? 2 : 4));
-  p.wchunk = chunk_of(keys, units * ((a.hd + kMaxDimsBlock - 1) / kMaxDimsBlock), 512, std::max(128u, 64 * p.splits));
+  p.wchunk = chunk_of(keys, units * ((a.hd + kMaxDimsBlock - 1) / kMaxDimsBlock), p.block_rows <= 16 ? 512 : 256, 64 * p.splits);
   p.wchunks = uint32_t((keys + p.wchunk - 1) / p.wchunk);
   uint64_t at = 0;
   auto take = [&](uint64_t bytes) {
@@ -882,7 +897,7 @@ uint64_t plan(const TreeArgs& a, const TreeSeq* seqs, const Group& g, Launch& p)
 
 template <int NSUB>
 void launch_scores(const Launch& p, uint32_t blocks, hipStream_t s) {
-  const uint32_t lds = p.block_rows / 16 * NSUB * 5 * kOp;
+  const uint32_t lds = p.block_rows / 16 * NSUB * 3 * kOp;
   auto go = [&](auto kernel) {
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 128 << 10);
     hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), lds, s, p);
@@ -931,7 +946,10 @@ void launch_tree_attention(const TreeArgs& a, const TreeSeq* seqs, uint32_t n, v
     if (p.block_rows <= 16) launch_wsum<1>(p, blocks(p.wchunks), s);
     else if (p.block_rows <= 32) launch_wsum<2>(p, blocks(p.wchunks), s);
     else launch_wsum<4>(p, blocks(p.wchunks), s);
-    hipLaunchKernelGGL(k_tree_join, dim3(p.rows, (a.hd + 63) / 64), dim3(256), 0, s, p);
+    if (p.wchunks * p.splits > 16)
+      hipLaunchKernelGGL(k_tree_join<4>, dim3(p.rows, (a.hd + 63) / 64), dim3(256), 0, s, p);
+    else
+      hipLaunchKernelGGL(k_tree_join<1>, dim3(p.rows, (a.hd + 255) / 256), dim3(256), 0, s, p);
   });
 }
 
