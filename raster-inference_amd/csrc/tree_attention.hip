@@ -12,8 +12,11 @@
 // cut into chunks over the grid at each step and the chunks' maxima, sums and
 // outputs (whole numbers: any order) joined by the next one:
 //   k_tree_scores   q.k on int8 MFMA -> scores, a maximum per (row, chunk)
-//   k_tree_terms    scores -> exp terms in place, a sum and a first maximum
-//   k_tree_wsum     terms -> weights, w.v on int8 MFMA -> partial sums
+//   k_tree_rows     scores of whole rows -> exp terms, their sum, weights; or, for
+//                   few long rows, over the chunks of each:
+//     k_tree_terms    scores -> terms in place, a sum and a first maximum
+//     k_tree_weights  terms -> weights
+//   k_tree_wsum     w.v on int8 MFMA -> partial sums
 //   k_tree_join     partial sums + residual * v[first maximum] -> out
 //
 // int32 values are taken apart into balanced base-256 digits, x = sum 256^j c_j
@@ -40,6 +43,7 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 constexpr uint32_t kSeqs = 32;  // sequences per launch (by value in the arguments)
 constexpr uint32_t kWaves = 8;
 constexpr uint32_t kThreads = 64 * kWaves;
+constexpr uint32_t kSumDims = 32 * kWaves;  // of a weighted-sum block
 constexpr uint32_t kOp = 1024;  // one MFMA operand: 64 lanes x 16 bytes
 
 // Sequence of a launch. Query rows of (sequence, kv head) are its drafted rows
@@ -55,21 +59,32 @@ struct Seq {
   uint32_t id0;      // row id of its first row
   uint32_t score_ld;
 };
+// What a row's output has besides its two-digit weights.
+struct RowEnd {
+  int64_t extra;     // times v of the first maximum: the residual
+  uint32_t first;    // the first maximum, kNone in a row that sees nothing
+  uint32_t n_big;    // keys of weights above 32639, at most two of a row: 65536
+  uint32_t big0, big1;  // times their v
+};
+constexpr uint32_t kNone = 0xffffffffu;
 struct Launch {
   TreeArgs a;
-  int32_t* scores;     // then the terms
+  int32_t* scores;     // of short rows then the weights, of long ones the terms
+  int8_t* weights;     // [score row][64 keys]: their weights' digits 0, then 1 (2 bytes a key)
   int32_t* pmax;       // [row id][chunks]
   int64_t* psum;
   uint32_t* pfirst;
   int64_t* planes;     // [plane][row id][hd]
-  int32_t* pweight;    // [row id][chunks of the weighted sums]
+  int32_t* pweight;    // [row id][chunks]
+  RowEnd* ends;        // [row id]
   uint32_t kv0, nkv;   // kv heads of the launch
   uint32_t n_seq, rows;  // row ids
   uint32_t chunk, chunks;    // keys per chunk of the scores and terms
   uint32_t wchunk, wchunks;  // of the weighted sums
   uint32_t splits, groups;   // waves of a weighted-sum block: key splits x groups of 32 dims
-  uint32_t row_blocks;
-  uint32_t block_rows;
+  uint32_t row_blocks, block_rows;  // of the scores
+  uint32_t sum_blocks, sum_rows;    // of the weighted sums
+  int whole;                 // rows are turned into weights whole
   int wide_k, wide_v;  // 16-byte aligned q and k rows, 8-byte aligned v rows
   Seq s[kSeqs];
 };
@@ -82,10 +97,10 @@ struct Item {
   uint32_t seq, kvh, chunk, rb;
   bool on;
 };
-__device__ inline Item item_of(const Launch& p, uint32_t chunks) {
-  const uint32_t id = blockIdx.x, w = (id / 8 / p.row_blocks) * 8 + id % 8;
+__device__ inline Item item_of(const Launch& p, uint32_t chunks, uint32_t row_blocks) {
+  const uint32_t id = blockIdx.x, w = (id / 8 / row_blocks) * 8 + id % 8;
   Item it;
-  it.rb = id / 8 % p.row_blocks;
+  it.rb = id / 8 % row_blocks;
   it.chunk = w % chunks;
   const uint32_t u = w / chunks;
   it.kvh = u % p.nkv;
@@ -215,7 +230,7 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 ? 4 : 2) void k_tree_scores(Lau
   __shared__ int32_t rmax[64];  // each row's largest score so far
   __shared__ Sight sight[64];
   __shared__ uint32_t qwide, last_start;
-  const Item it = item_of(p, p.chunks);
+  const Item it = item_of(p, p.chunks, p.row_blocks);
   if (!it.on) return;
   const Seq& s = p.s[it.seq];
   const TreeArgs& a = p.a;
@@ -385,13 +400,18 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 ? 4 : 2) void k_tree_scores(Lau
 // An exp term (at most 2^32, and otherwise below 2^32 - 65000) from its 32 bits.
 __device__ inline int64_t unpack_term(uint32_t e) { return int64_t(uint64_t(e) + (e == 0xffffffffu)); }
 
-// Terms: one wave per (row, chunk).
+// The sequence and place of a row id (wave-uniform).
+__device__ inline uint32_t seq_of(const Launch& p, uint32_t id) {
+  uint32_t b = 0;
+  while (b + 1 < p.n_seq && p.s[b + 1].id0 <= id) ++b;
+  return __builtin_amdgcn_readfirstlane(b);
+}
+
+// Terms of long rows: one wave per (row, chunk).
 __global__ __launch_bounds__(256) void k_tree_terms(Launch p) {
   const uint32_t l = threadIdx.x & 63, id = blockIdx.x * 4 + (threadIdx.x >> 6), chunk = blockIdx.y;
   if (id >= p.rows) return;
-  uint32_t b = 0;
-  while (b + 1 < p.n_seq && p.s[b + 1].id0 <= id) ++b;
-  const Seq& s = p.s[b];
+  const Seq& s = p.s[seq_of(p, id)];
   const uint32_t R = s.drafts * p.a.groups, local = id - s.id0, n = s.rows + s.drafts;
   const uint32_t k0 = chunk * p.chunk, k1 = min(k0 + p.chunk, n);
   if (k0 >= k1) return;
@@ -430,6 +450,7 @@ __global__ __launch_bounds__(256) void k_tree_terms(Launch p) {
   if (l == 0) {
     p.psum[uint64_t(id) * p.chunks + chunk] = int64_t(sum);
     p.pfirst[uint64_t(id) * p.chunks + chunk] = first;
+    if (chunk == 0) p.ends[id].n_big = 0;
   }
 }
 
@@ -463,148 +484,221 @@ __device__ __forceinline__ uint32_t weight_of(uint32_t e, uint32_t m, uint32_t s
   return y >> sh;
 }
 
+// Weights of four terms: their digits 0 and 1 (the bytes of (w + 0x8080) ^
+// 0x8080), a word each, their sum; keys of weights above 32639 go to `end` (their
+// digits are those of w - 65536).
+__device__ __forceinline__ uint2 weights4(const uint32_t (&e)[4], const Recip& rc, uint32_t key, int32_t& total, RowEnd* end) {
+  uint32_t w[4], unsure = 0;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    bool no;
+    w[q] = weight_of(e[q], rc.m, rc.sh, no);
+    unsure |= uint32_t(no) << q;
+  }
+#pragma unroll 1
+  for (; unsure; unsure &= unsure - 1) {
+    const int at = __builtin_ctz(unsure);
+    uint32_t x = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) x = q == at ? e[q] : x;
+    x = x ? uint32_t(softmax_weight(unpack_term(x), rc.sum)) : 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) w[q] = q == at ? x : w[q];
+  }
+  total += int32_t((w[0] + w[1]) + (w[2] + w[3]));
+  if (max(max(w[0], w[1]), max(w[2], w[3])) > 32639)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (w[q] > 32639) {
+        const uint32_t at = atomicAdd(&end->n_big, 1u);
+        if (at == 0) end->big0 = key + q;
+        if (at == 1) end->big1 = key + q;
+      }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) w[q] += 0x8080u;
+  const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), b = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+  return make_uint2(__builtin_amdgcn_perm(b, a, 0x05040100u) ^ 0x80808080u,
+                    __builtin_amdgcn_perm(b, a, 0x07060302u) ^ 0x80808080u);
+}
+// Where they go in a row of digits.
+__device__ __forceinline__ void put4(int8_t* row, uint32_t key, uint2 w) {
+  uint32_t* o = reinterpret_cast<uint32_t*>(row + (key >> 6) * 128 + (key & 63));
+  o[0] = w.x;
+  o[16] = w.y;
+}
+// The residual of a row: what its first maximum gets past its weight, with saturation.
+__device__ inline int64_t residual(int64_t total, int64_t sum) {
+  const int32_t w = softmax_weight(int64_t(1) << 32, sum);
+  return int64_t(add_sat(w, sub_sat(kOneAct, sat32(total)))) - w;
+}
+// Whole rows: W waves turn a row's scores into weights through LDS, four
+// consecutive keys per lane; the weights' digits replace the scores in place (from
+// the row's start on). With rows enough to fill the device this reads
+// the scores once and writes half their bytes, where terms and weights by chunks
+// read and write 2.5 times as much.
+constexpr uint32_t kRowKeys = 16384;  // most keys of a row (64 KB of terms)
+template <int W>
+__global__ __launch_bounds__(256) void k_tree_rows(Launch p, uint32_t lds_row) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t row_terms[];
+  __shared__ double red_sum[4];
+  __shared__ uint32_t red_first[4];
+  __shared__ int32_t red_total[4];
+  __shared__ RowEnd ends[4 / W];
+  const uint32_t l = threadIdx.x & 63, wave = threadIdx.x >> 6, in = wave / W, lane = threadIdx.x % (64 * W);
+  const uint32_t id = __builtin_amdgcn_readfirstlane(min(blockIdx.x * (4 / W) + in, p.rows - 1));
+  const bool on = blockIdx.x * (4 / W) + in < p.rows;
+  const Seq& s = p.s[seq_of(p, id)];
+  const uint32_t R = s.drafts * p.a.groups, local = id - s.id0, n = s.rows + s.drafts, n64 = (n + 63) & ~63u;
+  const uint32_t used = (n + p.chunk - 1) / p.chunk;
+  int32_t m = INT32_MIN;
+  for (uint32_t c = l; c < used; c += 64) m = max(m, p.pmax[uint64_t(id) * p.chunks + c]);
+  const Sight v = sight_of(p.a, s, local % R / p.a.groups);
+  m = int32_t(wave_max64(m));
+  int32_t* sc = p.scores + s.score0 + uint64_t(local) * s.score_ld;
+  uint32_t* terms = row_terms + in * lds_row;
+  if (lane == 0) ends[in].n_big = 0;
+  double sum = 0;  // (whole numbers below 2^53: exact in any order)
+  uint32_t first = kNone;
+  for (uint32_t k = 4 * lane; k < n64; k += 256 * W) {
+    const int4 t = *reinterpret_cast<const int4*>(sc + k);
+    const int32_t x[4] = {t.x, t.y, t.z, t.w};
+    uint32_t e[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint32_t gap = uint32_t(m) - uint32_t(x[q]);
+      const bool seen = gap < (1u << 20) && k + q < n && sees(v, s.rows, k + q);
+      double y = 0;
+      if (__any(seen)) {
+        y = seen ? softmax_term(gap) : 0.0;
+        if (seen && gap == 0) first = min(first, k + q);
+        sum += y;
+      }
+      e[q] = uint32_t(__builtin_fmin(y, 4294967295.0));  // (2^32: all ones, which no other term is)
+    }
+    *reinterpret_cast<uint4*>(terms + k) = make_uint4(e[0], e[1], e[2], e[3]);
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
+  first = ~uint32_t(wave_max64(int64_t(~first)));
+  if (l == 0) red_sum[wave] = sum, red_first[wave] = first;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    if (w == 0) sum = 0, first = kNone;
+    sum += red_sum[in * W + w];
+    first = min(first, red_first[in * W + w]);
+  }
+  const Recip rc = recip_of(int64_t(sum));
+  int32_t total = 0;
+  for (uint32_t k = 4 * lane; k < n64; k += 256 * W) {
+    const uint4 t = *reinterpret_cast<const uint4*>(terms + k);
+    const uint32_t e[4] = {t.x, t.y, t.z, t.w};
+    const uint2 w = weights4(e, rc, k, total, &ends[in]);
+    if (on) put4(reinterpret_cast<int8_t*>(sc), k, w);
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o, 64);
+  if (l == 0) red_total[wave] = total;
+  __syncthreads();
+  if (lane == 0 && on) {
+    int64_t all = 0;
+    for (int w = 0; w < W; ++w) all += red_total[in * W + w];
+    RowEnd end = ends[in];
+    end.first = first;
+    end.extra = first == kNone ? 0 : residual(all, rc.sum);
+    p.ends[id] = end;
+  }
+}
+
+// Weights of long rows: one wave per (row, chunk).
+__global__ __launch_bounds__(256) void k_tree_weights(Launch p) {
+  const uint32_t l = threadIdx.x & 63, id = blockIdx.x * 4 + (threadIdx.x >> 6), chunk = blockIdx.y;
+  if (id >= p.rows) return;
+  const Seq& s = p.s[seq_of(p, id)];
+  const uint32_t local = id - s.id0, n = s.rows + s.drafts, used = (n + p.chunk - 1) / p.chunk;
+  const uint32_t k0 = chunk * p.chunk, k2 = min((min(k0 + p.chunk, n) + 63) & ~63u, s.score_ld);
+  if (k0 >= n) return;
+  int64_t sum = 0;
+  for (uint32_t c = l; c < used; c += 64) sum += p.psum[uint64_t(id) * p.chunks + c];
+  const Recip rc = recip_of(wave_sum_wrap64(sum));
+  const uint64_t row = s.score0 + uint64_t(local) * s.score_ld;
+  int32_t total = 0;
+  for (uint32_t k = k0 + 4 * l; k < k2; k += 256) {
+    const uint4 t = *reinterpret_cast<const uint4*>(p.scores + row + k);
+    const uint32_t e[4] = {t.x, t.y, t.z, t.w};
+    put4(p.weights + 2 * row, k, weights4(e, rc, k, total, &p.ends[id]));
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o, 64);
+  if (l == 0) p.pweight[uint64_t(id) * p.chunks + chunk] = total;
+}
+
 // Weighted sums: a block takes up to 16 RT query rows, one chunk of keys and
-// 256 head dims; wave (dim group of 32, key split). Per step of 64 keys per
-// split the block turns the terms into weight digits in LDS, while each wave
-// loads the next values and multiplies the present ones. Lane 16 g + i of a
-// wave loads dims 2 i, 2 i + 1 of the keys 16 g + e: 128 consecutive bytes per
-// key.
-// Weights above 32639 (at most two of a row) need a third digit; they go on
-// without 65536, which is added from the list of their keys.
-constexpr uint32_t wsum_rounds(int RT) { return RT == 4 ? 1 : 2; }
-constexpr uint32_t most_splits(int RT) { return wsum_rounds(RT) * kThreads / (RT * 128); }
+// 256 head dims; each wave a group of 32 dims and a split of the keys, 64 of
+// them per step. Lane 16 g + i loads dims 2 i, 2 i + 1 of the keys 16 g + e (128
+// consecutive bytes per key) a step ahead. The weights' digits (128 bytes per row
+// and step) come through a ring of three LDS stages, copied two steps ahead: 1 KB
+// slots of eight rows, of whose 16-byte pieces piece q of row r lies at place q ^
+// (r >> 1 & 7), so that the 16 rows of an operand read hit different banks. (Every
+// wave loading the digits of all rows into registers took 122 us instead of ..)
+constexpr int kStages = 3;
 template <int RT>
 __global__ __launch_bounds__(kThreads, 2) void k_tree_wsum(Launch p) {
-  extern __shared__ __attribute__((aligned(16))) int8_t lds[];  // [2][split][query tile][digit][lane]
-  __shared__ Recip recip[16 * RT];
-  __shared__ uint32_t big_key[16 * RT][2], big_n[16 * RT];
-  __shared__ int32_t total[16 * RT];
-  __shared__ uint32_t vwide;
-  const Item it = item_of(p, p.wchunks);
+  extern __shared__ __attribute__((aligned(16))) int8_t ring[];  // [stage][split][row][128]
+  const Item it = item_of(p, p.wchunks, p.sum_blocks);
   if (!it.on) return;
   const Seq& s = p.s[it.seq];
   const TreeArgs& a = p.a;
-  const uint32_t R = s.drafts * a.groups, r0 = it.rb * p.block_rows, n = s.rows + s.drafts;
-  const uint32_t k0 = it.chunk * p.wchunk, k1 = min(k0 + p.wchunk, n);
-  if (r0 >= R || k0 >= k1) return;
-  const uint32_t rows = min(R - r0, p.block_rows), id0 = s.id0 + it.kvh * R + r0;
+  const uint32_t R = s.drafts * a.groups, r0 = it.rb * p.sum_rows, n = s.rows + s.drafts;
+  const uint32_t c0 = it.chunk * p.wchunk, c1 = min(c0 + p.wchunk, n);
+  if (r0 >= R || c0 >= c1) return;  // (workgroup-uniform)
   const uint32_t tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = l & 15, g = l >> 4;
-  const uint32_t kvh = p.kv0 + it.kvh, hd = a.hd, splits = p.splits, groups = p.groups;
-  const uint32_t split = wave / groups, dim0 = blockIdx.y * 256 + 32 * (wave % groups);
-  const int32_t* terms = p.scores + s.score0 + uint64_t(it.kvh * R + r0) * s.score_ld;
-  const uint32_t used = (n + p.chunk - 1) / p.chunk;
-  if (tid == 0) vwide = 0;
-  for (uint32_t r = wave; r < 16 * RT; r += kWaves) {
-    int64_t sum = 0;
-    if (r < rows)
-      for (uint32_t c = l; c < used; c += 64) sum += p.psum[uint64_t(id0 + r) * p.chunks + c];
-    sum = wave_sum_wrap64(sum);
-    if (l == 0) {
-      recip[r] = recip_of(sum);
-      big_n[r] = 0;
-      total[r] = 0;
-    }
-  }
-  __syncthreads();
-  const uint32_t per = 64 * splits;  // keys per step
-  // Weights of a step: eight keys of a row per thread and round, whose terms
-  // are loaded a step ahead.
-  constexpr uint32_t kRounds = wsum_rounds(RT);
-  const uint32_t items = splits * RT * 128;
-  auto load_terms = [&](uint32_t k, uint32_t u, uint32_t (&e)[8]) {
-    const uint32_t r = u / 8 % (16 * RT), key = k + 64 * (u / (128 * RT)) + 8 * (u % 8);
-    // (rows and keys past the end: any in range, not used)
-    const int4* src = reinterpret_cast<const int4*>(terms + uint64_t(min(r, rows - 1)) * s.score_ld + min(key, s.score_ld - 8));
-    const int4 t0 = src[0], t1 = src[1];
-    e[0] = uint32_t(t0.x), e[1] = uint32_t(t0.y), e[2] = uint32_t(t0.z), e[3] = uint32_t(t0.w);
-    e[4] = uint32_t(t1.x), e[5] = uint32_t(t1.y), e[6] = uint32_t(t1.z), e[7] = uint32_t(t1.w);
-  };
-  auto put_weights = [&](uint32_t k, uint32_t buf, uint32_t u, const uint32_t (&e)[8]) {
-    const uint32_t r = u / 8 % (16 * RT), sp = u / (128 * RT), o = u % 8, key = k + 64 * sp + 8 * o;
-    uint32_t w[8], d[2][2] = {{0, 0}, {0, 0}};
-    if (r < rows && key < k1) {
-      const uint32_t m = recip[r].m, sh = recip[r].sh;
-      uint32_t unsure = 0, most = 0;
-      int32_t tot = 0;
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        bool no;
-        w[q] = weight_of(e[q], m, sh, no);
-        unsure |= uint32_t(no) << q;
-      }
-#pragma unroll 1
-      for (; unsure; unsure &= unsure - 1) {
-        const int at = __builtin_ctz(unsure);
-        uint32_t x = 0;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) x = q == at ? e[q] : x;
-        x = x ? uint32_t(softmax_weight(unpack_term(x), recip[r].sum)) : 0;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) w[q] = q == at ? x : w[q];
-      }
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        tot += int32_t(w[q]);
-        most = max(most, w[q]);
-      }
-      if (most > 32639)
-#pragma unroll 1
-        for (int q = 0; q < 8; ++q) {
-          uint32_t x = 0;
-#pragma unroll
-          for (int c = 0; c < 8; ++c) x = q == c ? w[c] : x;
-          if (x > 32639) {
-            const uint32_t at = atomicAdd(&big_n[r], 1u);
-            if (at < 2) big_key[r][at] = key + q;
-          }
-        }
-      if (tot) {
-        if (blockIdx.y == 0) atomicAdd(&total[r], tot);
-        // digits of four weights at a time: bytes 0 and 1 of (w + 0x8080) ^ 0x8080
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t z[4];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) z[q] = w[4 * h + q] + 0x8080u;
-          const uint32_t a = __builtin_amdgcn_perm(z[1], z[0], 0x05010400u), b = __builtin_amdgcn_perm(z[3], z[2], 0x05010400u);
-          d[0][h] = __builtin_amdgcn_perm(b, a, 0x05040100u) ^ 0x80808080u;
-          d[1][h] = __builtin_amdgcn_perm(b, a, 0x07060302u) ^ 0x80808080u;
-        }
-      }
-    }
-    // lane 16 (o / 2) + r % 16, bytes 8 (o % 2) ..
-    int8_t* at = lds + (buf * splits * RT + sp * RT + r / 16) * 2 * kOp + (16 * (o / 2) + r % 16) * 16 + 8 * (o % 2);
-    *reinterpret_cast<uint2*>(at) = make_uint2(d[0][0], d[0][1]);
-    *reinterpret_cast<uint2*>(at + kOp) = make_uint2(d[1][0], d[1][1]);
-  };
+  const uint32_t kvh = p.kv0 + it.kvh, hd = a.hd, splits = p.splits;
+  const uint32_t split = wave / p.groups, dim0 = blockIdx.y * kSumDims + 32 * (wave % p.groups);
+  // the splits' equal shares of the chunk, in whole steps
+  const uint32_t steps = ((c1 - c0 + 63) / 64 + splits - 1) / splits;
+  const uint32_t k0 = c0 + split * steps * 64, k1 = min(k0 + steps * 64, c1);
+  const bool on = split < splits && dim0 < hd && k0 < k1;
+  const uint32_t rows = min(R - r0, p.sum_rows), id0 = s.id0 + it.kvh * R + r0;
   const uint64_t off = uint64_t(kvh) * hd;
-  const uint32_t dim = dim0 + 2 * i;
-  const bool dims_on = split < splits && dim0 < hd;  // (wave-uniform)
-  const uint32_t dim_in = dim + 1 < hd ? dim : (hd > 1 ? hd - 2 : 0);  // (sums of dims past hd are dropped)
+  const uint32_t dim = dim0 + 2 * i, dim_in = dim + 1 < hd ? dim : (hd > 1 ? hd - 2 : 0);  // (sums of dims past hd are dropped)
+  const uint32_t run_off = 16 * g * uint32_t(s.ld) + dim_in;
   auto load_v = [&](uint32_t k, int32_t (&x)[16][2]) {
-    if (!dims_on) return;
-    const uint32_t kk = k + 64 * split;
-    uint64_t at = s.first + kk;
+    uint64_t at = s.first + k;
     if (s.wrap && at >= s.wrap) at -= s.wrap;
-    if (p.wide_v && kk + 64 <= min(s.rows, k1) && (!s.wrap || at + 64 <= s.wrap) && s.ld < (1u << 22)) {
-      // whole substeps of one run of cached rows: scalar row addresses
-      const uint32_t o = 16 * g * uint32_t(s.ld) + dim_in;
+    if (p.wide_v && k + 64 <= s.rows && (!s.wrap || at + 64 <= s.wrap) && s.ld < (1u << 22)) {
+      // one run of cached rows: scalar row addresses
       const int32_t* base = s.v + at * s.ld + off;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         typedef int v2 __attribute__((ext_vector_type(2)));
-        const v2 t = *(global_ptr<const v2>)(to_global(base + e * s.ld) + o);
+        const v2 t = *(global_ptr<const v2>)(to_global(base + e * s.ld) + run_off);
         x[e][0] = t.x, x[e][1] = t.y;
       }
       return;
     }
-    // (weights are zero from k1 on)
+    // (weights are zero from the row's end on)
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const int32_t* row = row_ptr(s, s.v, a.v, a.kv_ld, min(kk + 16 * g + e, k1 - 1), off);
+      const int32_t* row = row_ptr(s, s.v, a.v, a.kv_ld, min(k + 16 * g + e, n - 1), off);
       x[e][0] = to_global(row)[min(dim, hd - 1)];
       x[e][1] = to_global(row)[min(dim + 1, hd - 1)];
       __builtin_amdgcn_sched_barrier(0);  // (one row's address at a time)
+    }
+  };
+  // this lane's pieces of the digits of step `st`: slot c of a split's 2 RT has rows 8 c ..
+  const uint64_t wrow = s.score0 + uint64_t(it.kvh * R + r0) * s.score_ld;
+  const int8_t* wbase = p.whole ? reinterpret_cast<const int8_t*>(p.scores + wrow) : p.weights + 2 * wrow;
+  const uint32_t wld = (p.whole ? 4 : 2) * s.score_ld;
+  const uint32_t slots = splits * RT * 2;
+  auto copy_w = [&](uint32_t st) {
+    for (uint32_t c = wave; c < slots; c += kWaves) {
+      const uint32_t r = 8 * (c % (2 * RT)) + l / 8, q = (l % 8) ^ (r >> 1 & 7);
+      // (rows past the last and steps past a share: in range, not used)
+      const uint32_t key = min(c0 + (c / (2 * RT) * steps + st) * 64, (n - 1) & ~63u);
+      __builtin_amdgcn_global_load_lds(
+          (const void __attribute__((address_space(1)))*)(wbase + uint64_t(min(r, rows - 1)) * wld + 2 * key + 16 * q),
+          (void __attribute__((address_space(3)))*)(ring + ((st % kStages) * slots + c) * kOp), 16, 0, 0);
     }
   };
   auto digit_words = [&](const int32_t (&x)[16][2], int c, v4i (&d)[4], uint32_t& all) {
@@ -617,6 +711,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_tree_wsum(Launch p) {
       for (int q = 0; q < 4; ++q) d[q][j] = int(w[q]);
     }
   };
+  // digit q of the 16 weights of row 16 T + i from key 16 g on, of stage `st`
+  const uint32_t place = split * RT * 2 * kOp + i * 128;
+  auto weights = [&](uint32_t st, int T, int q) {
+    return *reinterpret_cast<const v4i*>(ring + (st % kStages) * slots * kOp + place + T * 2048 +
+                                         16 * ((4 * q + g) ^ (i >> 1)));
+  };
   v4i acc[RT][2][4];
 #pragma unroll
   for (int T = 0; T < RT; ++T)
@@ -625,57 +725,50 @@ __global__ __launch_bounds__(kThreads, 2) void k_tree_wsum(Launch p) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) acc[T][c][q] = v4i{0, 0, 0, 0};
   int32_t x[16][2] = {};
-  uint32_t e[kRounds][8];
-  auto all_terms = [&](uint32_t k) {
-#pragma unroll
-    for (uint32_t c = 0; c < kRounds; ++c)
-      if (tid + kThreads * c < items) load_terms(k, tid + kThreads * c, e[c]);
+  uint32_t all = 0;
+  // every copy and load that a wave has in flight, then the workgroup
+  auto step_barrier = [&] {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0 | (7 << 4));  // vmcnt 0, lgkmcnt 0
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
   };
-  auto all_weights = [&](uint32_t k, uint32_t buf) {
-#pragma unroll
-    for (uint32_t c = 0; c < kRounds; ++c)
-      if (tid + kThreads * c < items) put_weights(k, buf, tid + kThreads * c, e[c]);
-  };
-  all_terms(k0);
-  load_v(k0, x);
-  all_weights(k0, 0);
-  if (k0 + per < k1) all_terms(k0 + per);
-  __syncthreads();
-  uint32_t all = 0, buf = 0;
-  for (uint32_t k = k0; k < k1; k += per, buf ^= 1) {
+  copy_w(0);
+  if (steps > 1) copy_w(1);
+  if (on) load_v(k0, x);
+#pragma unroll 1
+  for (uint32_t st = 0; st < steps; ++st) {
     v4i d[2][4];
     digit_words(x, 0, d[0], all);
     digit_words(x, 1, d[1], all);
-    if (k + per < k1) {
-      load_v(k + per, x);
-      all_weights(k + per, buf ^ 1);
-      if (k + 2 * per < k1) all_terms(k + 2 * per);
-    }
-    if (dims_on) {
-      const v4i* w = reinterpret_cast<const v4i*>(lds + (buf * splits + split) * RT * 2 * kOp);
 #pragma unroll
-      for (int T = 0; T < RT; ++T)
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int q = 0; q < 3; ++q) asm volatile("" : "+v"(d[c][q]));
+    step_barrier();
+    if (st + 2 < steps) copy_w(st + 2);
+    const uint32_t k = k0 + 64 * st;
+    if (on && k + 64 < k1) load_v(k + 64, x);
+    if (on && k < k1)
+#pragma unroll
+      for (int T = 0; T < RT; ++T) {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          const v4i wq = w[(T * 2 + q) * 64 + l];
+          const v4i w = weights(st, T, q);
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int j = 0; j < 3; ++j)
-              acc[T][c][q + j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wq, d[c][j], acc[T][c][q + j], 0, 0, 0);
-          __builtin_amdgcn_sched_barrier(0);
+              acc[T][c][q + j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, d[c][j], acc[T][c][q + j], 0, 0, 0);
         }
-    }
-    lds_barrier();  // (the next step's loads stay in flight)
+        __builtin_amdgcn_sched_barrier(0);
+      }
   }
-  if (all) vwide = 1;
-  __syncthreads();
   // lane l, component r: row 16 T + 4 g + r, dims dim and dim + 1
-  const uint32_t plane = it.chunk * splits + split;
-  int64_t* out = p.planes + (uint64_t(plane) * p.rows + id0) * hd;
+  const bool planes_on = split < splits && dim0 < hd;
+  int64_t* out = p.planes + (uint64_t(it.chunk * splits + split) * p.rows + id0) * hd;
   // the first `count` sums, sum q at digit q + shift
   auto put = [&](auto count, auto shift, bool add) {
-    if (!dims_on) return;
 #pragma unroll
     for (int T = 0; T < RT; ++T)
 #pragma unroll
@@ -688,60 +781,50 @@ __global__ __launch_bounds__(kThreads, 2) void k_tree_wsum(Launch p) {
             y[c] += uint64_t(int64_t(acc[T][c][q][r])) << (8 * (q + decltype(shift)::value));
         const uint32_t row = 16 * T + 4 * g + r;
         int64_t* o = out + uint64_t(row) * hd + dim;
-        if (row < rows && dim < hd) *o = int64_t((add ? uint64_t(*o) : 0) + y[0]);
-        if (row < rows && dim + 1 < hd) o[1] = int64_t((add ? uint64_t(o[1]) : 0) + y[1]);
+        if (planes_on && row < rows && dim < hd) *o = int64_t((add ? uint64_t(*o) : 0) + y[0]);
+        if (planes_on && row < rows && dim + 1 < hd) o[1] = int64_t((add ? uint64_t(o[1]) : 0) + y[1]);
       }
   };
   put(std::integral_constant<int, 4>(), std::integral_constant<int, 0>(), false);
-  if (blockIdx.y == 0 && tid < rows) p.pweight[uint64_t(id0 + tid) * p.wchunks + it.chunk] = total[tid];
-  __syncthreads();
-  // the 65536 that weights above 32639 went without (in the first split's plane)
-  const uint32_t d_end = min(hd, blockIdx.y * 256 + 256);
-  for (uint32_t r = wave; r < rows; r += kWaves)
-    for (uint32_t b = 0; b < min(big_n[r], 2u); ++b) {
-      const int32_t* v = row_ptr(s, s.v, a.v, a.kv_ld, big_key[r][b], off);
-      int64_t* o = p.planes + (uint64_t(it.chunk * splits) * p.rows + id0 + r) * hd;
-      for (uint32_t d = blockIdx.y * 256 + l; d < d_end; d += 64)
-        o[d] = int64_t(uint64_t(o[d]) + (uint64_t(int64_t(to_global(v)[d])) << 16));
-    }
-  __syncthreads();
-  if (!vwide) return;  // (workgroup-uniform)
-  // a value of the chunk is not narrow: its digits 3 and 4, in a pass of their own
+  if (!__syncthreads_or(all != 0)) return;
+  // a value of the block's is not narrow: digits 3 and 4, in a pass of their own
 #pragma unroll
   for (int T = 0; T < RT; ++T)
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int q = 0; q < 3; ++q) acc[T][c][q] = v4i{0, 0, 0, 0};
-  if (tid < 16 * RT) big_n[tid] = 2;  // (no more entries)
 #pragma unroll 1
-  for (uint32_t k = k0; k < k1; k += per) {
+  for (uint32_t st = 0; st < steps; ++st) {
+    const uint32_t k = k0 + 64 * st;
     __syncthreads();
-    all_terms(k);
-    all_weights(k, 0);
-    load_v(k, x);
-    __syncthreads();
-    if (!dims_on) continue;
-    const v4i* w = reinterpret_cast<const v4i*>(lds + split * RT * 2 * kOp);
+    copy_w(st);
+    if (on && k < k1) load_v(k, x);
+    step_barrier();
+    if (!on || k >= k1) continue;
+    v4i d[2][4], t[2];
+    uint32_t unused = 0;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      v4i d[4], t;
-      uint32_t unused = 0;
-      digit_words(x, c, d, unused);
+      digit_words(x, c, d[c], unused);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int32_t y[4] = {x[4 * j][c], x[4 * j + 1][c], x[4 * j + 2][c], x[4 * j + 3][c]};
-        t[j] = int(top4(y));
+        t[c][j] = int(top4(y));
       }
-#pragma unroll
-      for (int T = 0; T < RT; ++T)
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const v4i wq = w[(T * 2 + q) * 64 + l];
-          acc[T][c][q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wq, d[3], acc[T][c][q], 0, 0, 0);
-          acc[T][c][q + 1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wq, t, acc[T][c][q + 1], 0, 0, 0);
-        }
     }
+#pragma unroll
+    for (int T = 0; T < RT; ++T)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const v4i w = weights(st, T, q);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          acc[T][c][q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, d[c][3], acc[T][c][q], 0, 0, 0);
+          acc[T][c][q + 1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, t[c], acc[T][c][q + 1], 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
   }
   put(std::integral_constant<int, 3>(), std::integral_constant<int, 3>(), true);
 }
@@ -752,32 +835,28 @@ template <int SHARES>
 __global__ __launch_bounds__(256) void k_tree_join(Launch p) {
   const uint32_t l = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t id = blockIdx.x;
-  uint32_t b = 0;
-  while (b + 1 < p.n_seq && p.s[b + 1].id0 <= id) ++b;
-  const Seq& s = p.s[b];
+  const Seq& s = p.s[seq_of(p, id)];
   const TreeArgs& a = p.a;
   const uint32_t R = s.drafts * a.groups, local = id - s.id0, n = s.rows + s.drafts;
   const uint32_t kvh = p.kv0 + local / R, row = local % R, used = (n + p.chunk - 1) / p.chunk;
   const uint32_t wused = (n + p.wchunk - 1) / p.wchunk;
-  int64_t tot = 0, sum = 0;
-  uint32_t first = 0xffffffffu;
-  for (uint32_t c = l; c < used; c += 64) {
-    sum += p.psum[uint64_t(id) * p.chunks + c];
-    first = min(first, p.pfirst[uint64_t(id) * p.chunks + c]);
+  RowEnd end = p.ends[id];
+  if (!p.whole) {
+    int64_t total = 0, sum = 0;
+    uint32_t first = kNone;
+    for (uint32_t c = l; c < used; c += 64) {
+      sum += p.psum[uint64_t(id) * p.chunks + c];
+      first = min(first, p.pfirst[uint64_t(id) * p.chunks + c]);
+      total += p.pweight[uint64_t(id) * p.chunks + c];
+    }
+    sum = wave_sum_wrap64(sum);
+    total = wave_sum_wrap64(total);
+    end.first = ~uint32_t(wave_max64(int64_t(~first)));
+    end.extra = end.first == kNone ? 0 : residual(total, sum);
   }
-  for (uint32_t c = l; c < wused; c += 64) tot += p.pweight[uint64_t(id) * p.wchunks + c];
-  sum = wave_sum_wrap64(sum);
-  tot = wave_sum_wrap64(tot);
-  first = ~uint32_t(wave_max64(int64_t(~first)));
   int32_t* out = a.out + (s.row0 + row / a.groups) * a.out_ld + uint64_t(kvh * a.groups + row % a.groups) * a.hd;
-  int64_t extra = 0;
-  const int32_t* v = nullptr;
-  if (first != 0xffffffffu) {
-    // the residual goes to the first maximum, with saturation
-    const int32_t w = softmax_weight(int64_t(1) << 32, sum);
-    extra = int64_t(add_sat(w, sub_sat(kOneAct, sat32(tot)))) - w;
-    v = row_ptr(s, s.v, a.v, a.kv_ld, first, uint64_t(kvh) * a.hd);
-  }
+  const uint64_t off = uint64_t(kvh) * a.hd;
+  const int32_t* v = row_ptr(s, s.v, a.v, a.kv_ld, end.first == kNone ? n - 1 : end.first, off);
   const uint32_t d = 64 * (blockIdx.y * (4 / SHARES) + wave / SHARES) + l, in = min(d, a.hd - 1);
   const uint32_t planes = wused * p.splits;
   const int64_t* src = p.planes + uint64_t(id) * a.hd + in;
@@ -799,7 +878,11 @@ __global__ __launch_bounds__(256) void k_tree_join(Launch p) {
     if (wave) return;
     for (int w = 1; w < 4; ++w) y += share[w][l];
   }
-  if (d < a.hd) out[d] = v ? requant(int64_t(y + uint64_t(extra * to_global(v)[d]))) : 0;
+  if (d >= a.hd) return;
+  y += uint64_t(end.extra * to_global(v)[d]);
+  if (end.n_big > 0) y += uint64_t(int64_t(to_global(row_ptr(s, s.v, a.v, a.kv_ld, end.big0, off))[d])) << 16;
+  if (end.n_big > 1) y += uint64_t(int64_t(to_global(row_ptr(s, s.v, a.v, a.kv_ld, end.big1, off))[d])) << 16;
+  out[d] = end.first == kNone ? 0 : requant(int64_t(y));
 }
 
 uint64_t up(uint64_t v, uint64_t a) { return (v + a - 1) / a * a; }
@@ -809,7 +892,6 @@ struct Group {
   uint32_t b0, b1, kv0, nkv;
 };
 constexpr uint64_t kScoreBytes = uint64_t(256) << 20;  // score rows of a group (the Infinity Cache)
-constexpr uint32_t kMaxDimsBlock = 256;
 
 uint32_t score_ld(const TreeSeq& s) { return uint32_t(up(uint64_t(s.rows) + s.drafts, 64)); }
 uint64_t seq_score_bytes(const TreeArgs& a, const TreeSeq& s) { return uint64_t(s.drafts) * a.groups * score_ld(s) * 4; }
@@ -869,16 +951,21 @@ uint64_t plan(const TreeArgs& a, const TreeSeq* seqs, const Group& g, Launch& p)
   }
   p.wide_k = w4;
   p.wide_v = w2;
-  // 64 query rows per block; 32 where their digits would take more than half the
-  // LDS, or where the waves of a weighted-sum block share the keys instead of the dims
-  p.block_rows = std::min<uint32_t>(uint32_t(up(most, 16)), a.hd > 128 && a.hd <= 256 ? 64 : 32);
+  // 64 query rows per block; 32 where their digits or their sums' registers would
+  // leave the device half empty
+  p.block_rows = std::min<uint32_t>(uint32_t(up(most, 16)), a.hd <= 256 ? 64 : 32);
   p.row_blocks = (most + p.block_rows - 1) / p.block_rows;
   units = uint64_t(p.n_seq) * g.nkv * p.row_blocks;
   p.chunk = chunk_of(keys, units, 512, 16 * kWaves);
   p.chunks = uint32_t((keys + p.chunk - 1) / p.chunk);
+  p.whole = keys <= kRowKeys && (p.rows >= 256 || keys <= 4096);
   p.groups = a.hd <= 32 ? 1 : a.hd <= 64 ? 2 : a.hd <= 128 ? 4 : 8;
-  p.splits = std::min(kWaves / p.groups, most_splits(p.block_rows <= 16 ? 1 : p.block_rows <= 32 ? 2 : 4));
-  p.wchunk = chunk_of(keys, units * ((a.hd + kMaxDimsBlock - 1) / kMaxDimsBlock), p.block_rows <= 16 ? 512 : 256, 64 * p.splits);
+  p.splits = kWaves / p.groups;
+  p.sum_rows = std::min<uint32_t>(uint32_t(up(most, 16)), a.hd <= 64 ? 32 : 64);
+  p.sum_blocks = (most + p.sum_rows - 1) / p.sum_rows;
+  const uint64_t sums = uint64_t(p.n_seq) * g.nkv * p.sum_blocks * ((a.hd + kSumDims - 1) / kSumDims);
+  p.wchunk = chunk_of(keys, sums, 256, 64);
+  p.splits = std::min(p.splits, p.wchunk / 64);
   p.wchunks = uint32_t((keys + p.wchunk - 1) / p.wchunk);
   uint64_t at = 0;
   auto take = [&](uint64_t bytes) {
@@ -891,7 +978,9 @@ uint64_t plan(const TreeArgs& a, const TreeSeq* seqs, const Group& g, Launch& p)
   p.psum = reinterpret_cast<int64_t*>(take(uint64_t(p.rows) * p.chunks * 8));
   p.pfirst = reinterpret_cast<uint32_t*>(take(uint64_t(p.rows) * p.chunks * 4));
   p.planes = reinterpret_cast<int64_t*>(take(uint64_t(p.wchunks) * p.splits * p.rows * a.hd * 8));
-  p.pweight = reinterpret_cast<int32_t*>(take(uint64_t(p.rows) * p.wchunks * 4));
+  p.pweight = reinterpret_cast<int32_t*>(take(uint64_t(p.rows) * p.chunks * 4));
+  p.ends = reinterpret_cast<RowEnd*>(take(uint64_t(p.rows) * sizeof(RowEnd)));
+  p.weights = reinterpret_cast<int8_t*>(take(p.whole ? 0 : scores * 2));
   return at;
 }
 
@@ -908,11 +997,21 @@ void launch_scores(const Launch& p, uint32_t blocks, hipStream_t s) {
 }
 template <int RT>
 void launch_wsum(const Launch& p, uint32_t blocks, hipStream_t s) {
-  const uint32_t lds = 2 * p.splits * RT * 2 * kOp;
-  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_tree_wsum<RT>),
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, 128 << 10);
-  (void)attr;
-  hipLaunchKernelGGL(k_tree_wsum<RT>, dim3(blocks, (p.a.hd + kMaxDimsBlock - 1) / kMaxDimsBlock), dim3(kThreads), lds, s, p);
+  (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&k_tree_wsum<RT>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                            128 << 10);
+  hipLaunchKernelGGL(k_tree_wsum<RT>, dim3(blocks, (p.a.hd + kSumDims - 1) / kSumDims), dim3(kThreads),
+                     kStages * p.splits * RT * 2 * kOp, s, p);
+}
+void launch_rows(const Launch& p, hipStream_t s) {
+  uint32_t ld = 0;
+  for (uint32_t b = 0; b < p.n_seq; ++b) ld = std::max(ld, p.s[b].score_ld);
+  if (ld <= 1024) {
+    hipLaunchKernelGGL(k_tree_rows<1>, dim3((p.rows + 3) / 4), dim3(256), 4 * ld * 4, s, p, ld);
+  } else {
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&k_tree_rows<4>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                              kRowKeys * 4);
+    hipLaunchKernelGGL(k_tree_rows<4>, dim3(p.rows), dim3(256), ld * 4, s, p, ld);
+  }
 }
 
 }  // namespace
@@ -934,18 +1033,24 @@ void launch_tree_attention(const TreeArgs& a, const TreeSeq* seqs, uint32_t n, v
       q = reinterpret_cast<std::remove_reference_t<decltype(q)>>(static_cast<uint8_t*>(work) + reinterpret_cast<uintptr_t>(q));
     };
     place(p.scores), place(p.pmax), place(p.psum), place(p.pfirst), place(p.planes), place(p.pweight);
+    place(p.ends), place(p.weights);
     const uint32_t units = p.n_seq * p.nkv;
-    auto blocks = [&](uint32_t chunks) { return uint32_t(up(uint64_t(units) * chunks, 8)) * p.row_blocks; };
+    auto blocks = [&](uint32_t chunks) { return uint32_t(up(uint64_t(units) * chunks, 8)); };
     const uint32_t nsub = (a.hd + 63) / 64;
-    if (nsub == 1) launch_scores<1>(p, blocks(p.chunks), s);
-    else if (nsub == 2) launch_scores<2>(p, blocks(p.chunks), s);
-    else if (nsub == 3) launch_scores<3>(p, blocks(p.chunks), s);
-    else if (nsub == 4) launch_scores<4>(p, blocks(p.chunks), s);
-    else launch_scores<8>(p, blocks(p.chunks), s);
-    hipLaunchKernelGGL(k_tree_terms, dim3((p.rows + 3) / 4, p.chunks), dim3(256), 0, s, p);
-    if (p.block_rows <= 16) launch_wsum<1>(p, blocks(p.wchunks), s);
-    else if (p.block_rows <= 32) launch_wsum<2>(p, blocks(p.wchunks), s);
-    else launch_wsum<4>(p, blocks(p.wchunks), s);
+    if (nsub == 1) launch_scores<1>(p, blocks(p.chunks) * p.row_blocks, s);
+    else if (nsub == 2) launch_scores<2>(p, blocks(p.chunks) * p.row_blocks, s);
+    else if (nsub == 3) launch_scores<3>(p, blocks(p.chunks) * p.row_blocks, s);
+    else if (nsub == 4) launch_scores<4>(p, blocks(p.chunks) * p.row_blocks, s);
+    else launch_scores<8>(p, blocks(p.chunks) * p.row_blocks, s);
+    if (p.whole) {
+      launch_rows(p, s);
+    } else {
+      hipLaunchKernelGGL(k_tree_terms, dim3((p.rows + 3) / 4, p.chunks), dim3(256), 0, s, p);
+      hipLaunchKernelGGL(k_tree_weights, dim3((p.rows + 3) / 4, p.chunks), dim3(256), 0, s, p);
+    }
+    if (p.sum_rows <= 16) launch_wsum<1>(p, blocks(p.wchunks) * p.sum_blocks, s);
+    else if (p.sum_rows <= 32) launch_wsum<2>(p, blocks(p.wchunks) * p.sum_blocks, s);
+    else launch_wsum<4>(p, blocks(p.wchunks) * p.sum_blocks, s);
     if (p.wchunks * p.splits > 16)
       hipLaunchKernelGGL(k_tree_join<4>, dim3(p.rows, (a.hd + 63) / 64), dim3(256), 0, s, p);
     else
