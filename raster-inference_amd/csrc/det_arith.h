@@ -331,31 +331,32 @@ DET_HD int64_t softmax_exp(int32_t logit, int32_t max_logit) {
   return rshift_rte(t, unsigned(shift));  // shift <= 23 here
 }
 
+// Whole numbers held in doubles: round(a b), ties to even, of a product below
+// 2^51. The multiply-add rounds the exact a b + 1.5 2^52 once, to a whole number.
+DET_HD double mul_rint(double a, double b) {
+  constexpr double kWhole = 6755399441055744.0;  // 1.5 2^52
+  return __builtin_fma(a, b, kWhole) - kWhole;
+}
+// round(v / d), ties to even, as the rounded product with the nearest double to
+// 1 / d: exact for d = 2, 6, 24, 120, 720 and 5040 and every whole v below 2^32
+// (softmax) or 24 2^32 (sine and cosine): the product is off by less than 2^-17,
+// no quotient but a tie is nearer than that to a half, and at every tie in those
+// ranges the product comes out as the half itself (all of them were tried).
+template <int D>
+DET_HD double div_rint(double v) {
+  return __builtin_rint(v * (1.0 / D));
+}
+
 // softmax_exp(logit, max_logit) of a gap d = max_logit - logit below 2^20, as
-// the double that it is exactly (a whole number of at most 2^32), in about 35
-// instructions against 140: d 2^16 / ln2 and its remainder from one high
-// product; the powers' rounded products from multiply-adds with half a unit (a
-// tie leaves a zero low word: softmax_exp itself then decides); the quotients by
-// 2, 6, 24 and 120 as rounded products with the divisors' reciprocals, the sum
-// and its shift in double arithmetic, whose rounding is half to even. That
-// every quotient has the exact rounding, ties among them, was checked for every
-// value the powers take; the sums are whole numbers below 2^34.
-// k_tree_terms at 4096 rows of 8256 keys: 126 -> 61 us.
+// the double that it is exactly (a whole number of at most 2^32), in about 32
+// instructions against 140: d 2^16 / ln2 from one high product (exact for every
+// d), then the series and the shift with softmax_exp's roundings in double
+// arithmetic. k_tree_rows at 4096 rows of 8256 keys spent 126 us on softmax_exp.
 DET_HD double softmax_term(uint32_t d) {
   const uint32_t shift = uint32_t((uint64_t(d << 12) * 3098164009u) >> 32) >> 27;
-  const uint32_t r1 = (d << 16) - shift * 2977044472u;
-  const uint64_t half = 0x80000000u;
-  const uint64_t p2 = uint64_t(r1) * r1 + half;
-  const uint32_t r2 = uint32_t(p2 >> 32);
-  const uint64_t p3 = uint64_t(r2) * r1 + half;
-  const uint32_t r3 = uint32_t(p3 >> 32);
-  const uint64_t p4 = uint64_t(r3) * r1 + half;
-  const uint32_t r4 = uint32_t(p4 >> 32);
-  const uint64_t p5 = uint64_t(r4) * r1 + half;
-  const uint32_t r5 = uint32_t(p5 >> 32);
-  if (!uint32_t(p2) | !uint32_t(p3) | !uint32_t(p4) | !uint32_t(p5)) return double(softmax_exp(0, int32_t(d)));
-  const double t = (4294967296.0 - double(r1)) + (__builtin_rint(double(r2) * 0.5) - __builtin_rint(double(r3) * (1.0 / 6))) +
-                   (__builtin_rint(double(r4) * (1.0 / 24)) - __builtin_rint(double(r5) * (1.0 / 120)));
+  const double r1 = double((d << 16) - shift * 2977044472u), r = r1 * 0x1p-32;
+  const double r2 = mul_rint(r1, r), r3 = mul_rint(r2, r), r4 = mul_rint(r3, r), r5 = mul_rint(r4, r);
+  const double t = (4294967296.0 - r1) + (div_rint<2>(r2) - div_rint<6>(r3)) + (div_rint<24>(r4) - div_rint<120>(r5));
   return __builtin_rint(__builtin_ldexp(t, -int(shift)));
 }
 
@@ -483,6 +484,25 @@ DET_HD void sin_cos(int64_t angle, int32_t* c, int32_t* s) {
   int32_t sv = requant(sin_poly(q)), cv = requant(cos_poly(q));
   *s = sneg ? neg_sat32(sv) : sv;
   *c = cneg ? neg_sat32(cv) : cv;
+}
+// sin_cos with the polynomials in double arithmetic: the same roundings (the
+// reduced angle is at most 2^32.7 and every power of it below 24 2^32), about 80
+// instructions against 800.
+DET_HD void sin_cos_rint(int64_t angle, int32_t* c, int32_t* s) {
+  const int64_t HALF_PI = 6746518852ll, PI = 13493037705ll, THREE_HALF_PI = 20239556557ll, TWO_PI = 26986075409ll;
+  int64_t red = angle % TWO_PI;
+  if (red < 0) red += TWO_PI;
+  const bool sneg = red > PI, cneg = red > HALF_PI && red <= THREE_HALF_PI;
+  const int64_t q = red <= HALF_PI ? red : (red <= PI ? PI - red : (red <= THREE_HALF_PI ? red - PI : TWO_PI - red));
+  const double x = double(q), y = x * 0x1p-32;
+  const double x2 = mul_rint(x, y), y2 = x2 * 0x1p-32;
+  const double x3 = mul_rint(x2, y), x5 = mul_rint(x3, y2), x7 = mul_rint(x5, y2);
+  const double x4 = mul_rint(x2, y2), x6 = mul_rint(x4, y2);
+  const double sn = (x - div_rint<6>(x3)) + (div_rint<120>(x5) - div_rint<5040>(x7));
+  const double cs = (4294967296.0 - div_rint<2>(x2)) + (div_rint<24>(x4) - div_rint<720>(x6));
+  const int32_t sv = int32_t(__builtin_rint(sn * 0x1p-16)), cv = int32_t(__builtin_rint(cs * 0x1p-16));
+  *s = sneg ? -sv : sv;
+  *c = cneg ? -cv : cv;
 }
 // RoPE angle = position * inv_freq, clamped to i64 (ops.rs:613-617).
 DET_HD int64_t rope_angle(uint64_t position, int64_t inv_freq) {

@@ -6,6 +6,8 @@
 // cosine and sine of position * frequency (times the amplitude).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "det_arith.h"
 #include "verify.h"
 #include "wave.h"
@@ -33,116 +35,145 @@ struct Vec<4> {
 };
 
 // One workgroup per token: its threads compute the token's cosines and sines
-// once into LDS, then each group of `lanes` lanes takes one head row at a
-// time, V consecutive values per lane and step, E steps. A pair of the half
-// layout meets through the wave's LDS row; an interleaved pair sits in one
-// lane (V = 4) or in neighbouring ones.
-template <int V, int E>
-__global__ __launch_bounds__(512) void k_head_rope(HeadRopeArgs a, uint32_t lanes) {
-  extern __shared__ __attribute__((aligned(16))) int32_t lds[];  // cosines, sines, a row per lane group
+// once into LDS, then each group of `lanes` lanes takes up to U head rows at a
+// time, V consecutive values per lane and step, E steps; the first rows' loads
+// are on their way while the cosines are computed. A pair of the half layout
+// meets through the rows' LDS copies, an interleaved pair in one lane (V = 4) or
+// through them as well.
+template <int V, int E, int U>
+__global__ __launch_bounds__(256) void k_head_rope(HeadRopeArgs a, uint32_t lanes) {
+  extern __shared__ __attribute__((aligned(16))) int32_t lds[];  // cosines, sines, U rows per lane group
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
   const uint32_t per_wave = 64 / lanes, li = lane % lanes, hd = a.hd, pairs = a.pairs;
+  const uint32_t table = (pairs + 3) & ~3u, row_ld = (hd + 3) & ~3u;
   const uint64_t t = blockIdx.x;
   int32_t* cs = lds;
-  int32_t* sn = lds + ((pairs + 3) & ~3u);
-  int32_t* row = lds + 2 * ((pairs + 3) & ~3u) + (wave * per_wave + lane / lanes) * ((hd + 3) & ~3u);
-  if (pairs) {
-    const uint64_t pos = a.positions[t];
-    for (uint32_t i = tid; i < pairs; i += blockDim.x) {
-      int32_t c, s;
-      sin_cos(rope_angle(pos, a.freq[i]), &c, &s);
-      cs[i] = a.amplitude == kOneAct ? c : mul_sat(c, a.amplitude);
-      sn[i] = a.amplitude == kOneAct ? s : mul_sat(s, a.amplitude);
-    }
-    __syncthreads();
-  }
-  for (uint32_t r0 = wave * per_wave; r0 < a.total; r0 += waves * per_wave) {
-    const uint32_t r = r0 + lane / lanes;
-    const bool on = r < a.total;
-    // the row's set and head
-    uint32_t h = on ? r : 0;
-    HeadSet s = a.set[0];
+  int32_t* sn = lds + table;
+  int32_t* row = lds + 2 * table + (wave * per_wave + lane / lanes) * U * row_ld;
+  const bool meet = !(V == 4 && a.interleaved);  // pairs meet in LDS
+  const uint32_t step = waves * per_wave;
+  for (uint32_t r0 = wave * per_wave;; r0 += step * U) {
+    const bool turn = r0 == wave * per_wave;  // (every wave's first round)
+    if (!turn && r0 >= a.total) break;
+    // the rows' sets and heads, their values
+    HeadSet s[U];
+    const int32_t* src[U];
+    int32_t* dst[U];
+    bool on[U];
+    int32_t x[U][E][V];
 #pragma unroll
-    for (uint32_t q = 1; q < kHeadSets; ++q)
-      if (q < a.n_sets && h >= s.heads) {
-        h -= s.heads;
-        s = a.set[q];
+    for (int u = 0; u < U; ++u) {
+      const uint32_t r = r0 + u * step + lane / lanes;
+      on[u] = r < a.total;
+      uint32_t h = on[u] ? r : 0;
+      s[u] = a.set[0];
+#pragma unroll
+      for (uint32_t q = 1; q < kHeadSets; ++q)
+        if (q < a.n_sets && h >= s[u].heads) {
+          h -= s[u].heads;
+          s[u] = a.set[q];
+        }
+      src[u] = s[u].x + t * s[u].ld + uint64_t(h) * hd;
+      dst[u] = s[u].out + t * s[u].out_ld + uint64_t(h) * hd;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const uint32_t c = V * (li + 64 * e);
+#pragma unroll
+        for (int v = 0; v < V; ++v) x[u][e][v] = 0;
+        if (on[u] && c < hd) Vec<V>::load(src[u] + c, x[u][e]);
       }
-    const int32_t* src = s.x + t * s.ld + uint64_t(h) * hd;
-    int32_t* dst = s.out + t * s.out_ld + uint64_t(h) * hd;
-    int32_t x[E][V];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const uint32_t c = V * (li + 64 * e);
-#pragma unroll
-      for (int v = 0; v < V; ++v) x[e][v] = 0;
-      if (on && c < hd) Vec<V>::load(src + c, x[e]);
     }
-    if (s.flags & 1) {
+    if (turn && pairs) {
+      const uint64_t pos = a.positions[t];
+      for (uint32_t i = tid; i < pairs; i += blockDim.x) {
+        int32_t c, sv;
+        sin_cos_rint(rope_angle(pos, a.freq[i]), &c, &sv);
+        cs[i] = a.amplitude == kOneAct ? c : mul_sat(c, a.amplitude);
+        sn[i] = a.amplitude == kOneAct ? sv : mul_sat(sv, a.amplitude);
+      }
+      lds_barrier();
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (!(s[u].flags & 1)) continue;
       // (non-negative terms: the saturating sum is the least of the sum and i64::MAX in any order)
       int64_t ss = 0;
 #pragma unroll
       for (int e = 0; e < E; ++e)
 #pragma unroll
-        for (int v = 0; v < V; ++v) ss = add_sat64_nn(ss, sq_term(x[e][v]));
-      for (uint32_t off = 1; off < lanes; off <<= 1) ss = add_sat64_nn(ss, __shfl_xor(ss, int(off), 64));
+        for (int v = 0; v < V; ++v) ss = add_sat64_nn(ss, sq_term(x[u][e][v]));
+      if (lanes == 64) ss = wave_sum_sat64(ss);
+      else
+        for (uint32_t off = 1; off < lanes; off <<= 1) ss = add_sat64_nn(ss, __shfl_xor(ss, int(off), 64));
       const int32_t scale = rms_scale_from_sumsq(ss, hd, a.eps);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const uint32_t c = V * (li + 64 * e);
         if (c >= hd) continue;
         int32_t g[V];
-        if (s.gain) Vec<V>::load(s.gain + c, g);
+        if (s[u].gain) Vec<V>::load(s[u].gain + c, g);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          x[e][v] = mul_sat(x[e][v], scale);
-          if (s.gain) x[e][v] = mul_sat(x[e][v], g[v]);
+          x[u][e][v] = mul_sat(x[u][e][v], scale);
+          if (s[u].gain) x[u][e][v] = mul_sat(x[u][e][v], g[v]);
         }
       }
     }
-    if (pairs && __any(s.flags & 2)) {
-      wave_lds_sync();  // the previous rows have been read
+    if (pairs) {
+      if (meet) {
+        wave_lds_sync();  // the previous round's rows have been read
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const uint32_t c = V * (li + 64 * e);
-        if (c < hd) Vec<V>::store(row + c, x[e]);
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const uint32_t c = V * (li + 64 * e);
+            if (c < hd && (s[u].flags & 2)) Vec<V>::store(row + u * row_ld + c, x[u][e]);
+          }
+        wave_lds_sync();
       }
-      wave_lds_sync();
-      if (s.flags & 2) {
 #pragma unroll
-        for (int e = 0; e < E; ++e)
+      for (int u = 0; u < U; ++u) {
+        if (!(s[u].flags & 2)) continue;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          int32_t y[V];
 #pragma unroll
           for (int v = 0; v < V; ++v) {
             const uint32_t c = V * (li + 64 * e) + v;
+            y[v] = x[u][e][v];
             if (c >= 2 * pairs) continue;
             const bool second = a.interleaved ? (c & 1) : c >= pairs;
             const uint32_t i = a.interleaved ? c >> 1 : (second ? c - pairs : c);
-            const int32_t other = row[a.interleaved ? (c ^ 1) : (second ? c - pairs : c + pairs)];
-            const int32_t p = mul_sat(x[e][v], cs[i]), q = mul_sat(other, sn[i]);
-            x[e][v] = second ? add_sat(p, q) : sub_sat(p, q);
+            const int32_t other =
+                meet ? row[u * row_ld + (a.interleaved ? (c ^ 1) : (second ? c - pairs : c + pairs))] : x[u][e][v ^ (V > 1)];
+            const int32_t p = mul_sat(x[u][e][v], cs[i]), q = mul_sat(other, sn[i]);
+            y[v] = second ? add_sat(p, q) : sub_sat(p, q);
           }
+#pragma unroll
+          for (int v = 0; v < V; ++v) x[u][e][v] = y[v];
+        }
       }
     }
-    if (on)
+#pragma unroll
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const uint32_t c = V * (li + 64 * e);
-        if (c < hd) Vec<V>::store(dst + c, x[e]);
+        if (on[u] && c < hd) Vec<V>::store(dst[u] + c, x[u][e]);
       }
   }
 }
 
-template <int V, int E>
+template <int V, int E, int U>
 void launch(const HeadRopeArgs& a, hipStream_t s) {
   uint32_t lanes = 64;
   if (E == 1)
     while (lanes > 1 && lanes / 2 * V >= a.hd) lanes /= 2;
   const uint32_t per_wave = 64 / lanes;
-  uint32_t waves = (a.total + per_wave - 1) / per_wave;
-  if (waves > 4) waves = 4;
-  if (waves < 2 && a.pairs > 64) waves = 2;
-  const size_t bytes = (2 * ((a.pairs + 3) & ~3u) + waves * per_wave * ((a.hd + 3) & ~3u)) * 4;
-  hipLaunchKernelGGL((k_head_rope<V, E>), dim3(unsigned(a.rows)), dim3(64 * waves), bytes, s, a, lanes);
+  uint32_t waves = (a.total + per_wave * U - 1) / (per_wave * U);
+  waves = std::min(std::max(waves, a.pairs > 64 ? 2u : 1u), 4u);
+  const size_t bytes = (2 * ((a.pairs + 3) & ~3u) + waves * per_wave * U * ((a.hd + 3) & ~3u)) * 4;
+  hipLaunchKernelGGL((k_head_rope<V, E, U>), dim3(unsigned(a.rows)), dim3(64 * waves), bytes, s, a, lanes);
 }
 
 }  // namespace
@@ -157,13 +188,13 @@ void launch_head_rope(const HeadRopeArgs& a, hipStream_t s) {
              reinterpret_cast<uintptr_t>(h.gain)) & 15) == 0;
   }
   if (wide) {
-    if (a.hd <= 256) launch<4, 1>(a, s);
-    else if (a.hd <= 512) launch<4, 2>(a, s);
-    else launch<4, 4>(a, s);
+    if (a.hd <= 256) launch<4, 1, 3>(a, s);
+    else if (a.hd <= 512) launch<4, 2, 3>(a, s);
+    else launch<4, 4, 1>(a, s);
   } else {
-    if (a.hd <= 64) launch<1, 1>(a, s);
-    else if (a.hd <= 256) launch<1, 4>(a, s);
-    else launch<1, 16>(a, s);
+    if (a.hd <= 64) launch<1, 1, 3>(a, s);
+    else if (a.hd <= 256) launch<1, 4, 2>(a, s);
+    else launch<1, 16, 1>(a, s);
   }
 }
 

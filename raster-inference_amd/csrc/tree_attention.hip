@@ -211,7 +211,10 @@ __device__ __forceinline__ void score_tile(const v4i (&k)[NSUB][3], const v4i* q
     const uint32_t q = uint32_t(v) + (uint32_t(acc[3][r]) << 8) + (uint32_t(acc[4][r]) << 16);
     out[r] = int32_t(q + uint32_t(rem + (q & 1u) > 0x8000u));
   }
-  if (__any(far != 0))
+  if (__any(far != 0)) {
+    // (a branch in earnest: the 64-bit sums would be computed in any case)
+#pragma unroll
+    for (int s = 0; s < 5; ++s) asm volatile("" : "+v"(acc[s]));
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       uint64_t dot = 0;
@@ -219,6 +222,7 @@ __device__ __forceinline__ void score_tile(const v4i (&k)[NSUB][3], const v4i* q
       for (int s = 0; s < 5; ++s) dot += uint64_t(int64_t(acc[s][r])) << (8 * s);
       out[r] = requant(int64_t(dot));
     }
+  }
 }
 
 // Scores: a block takes up to 64 query rows (digits in LDS, converted once) and
@@ -563,13 +567,22 @@ __global__ __launch_bounds__(256) void k_tree_rows(Launch p, uint32_t lds_row) {
     const int4 t = *reinterpret_cast<const int4*>(sc + k);
     const int32_t x[4] = {t.x, t.y, t.z, t.w};
     uint32_t e[4];
+    // what of the four keys is seen
+    uint32_t vis = k >= v.start && k + 4 <= s.rows ? 15u : 0u;
+    if (__any(vis == 0)) {
+      asm volatile("");
+      vis = 0;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) vis |= uint32_t(k + q < n && sees(v, s.rows, k + q)) << q;
+    }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const uint32_t gap = uint32_t(m) - uint32_t(x[q]);
-      const bool seen = gap < (1u << 20) && k + q < n && sees(v, s.rows, k + q);
+      const bool seen = gap < (1u << 20) && ((vis >> q) & 1u);
       double y = 0;
       if (__any(seen)) {
-        y = seen ? softmax_term(gap) : 0.0;
+        y = softmax_term(seen ? gap : (1u << 20) - 1);
+        y = seen ? y : 0.0;
         if (seen && gap == 0) first = min(first, k + q);
         sum += y;
       }

@@ -79,6 +79,26 @@ int main(int argc, char** argv) {
     if (d > 0 && o > int64_t((1ull << 32) - (1ull << 16))) bad++;
   }
   report("softmax_exp_all_gaps", nexp, bad);
+  // softmax_term over every gap that it takes, against the oracle's term
+  bad = 0;
+  for (int64_t d = 0; d < (1 << 20); ++d) {
+    int64_t o;
+    orc_attention_softmax_exp_term(int32_t(-d), 0, &o);
+    if (det::softmax_term(uint32_t(d)) != double(o)) { bad++; if (bad < 5) printf("  softmax_term d=%lld\n", (long long)d); }
+  }
+  report("softmax_term_all_gaps", 1 << 20, bad);
+  // sin_cos_rint: every quarter-turn border, random angles of all sizes
+  bad = 0;
+  long nsc = 0;
+  for (int64_t k = 0; k < 400000; ++k, ++nsc) {
+    const int64_t quarter = 6746518852ll + (k & 3) * 6746518852ll;
+    const int64_t a = k < 40000 ? quarter * (1 + (k >> 2) % 7) + (k % 601) - 300 : (k & 1 ? int64_t(rng() % 26986075409ull) : pick64());
+    int32_t oc, os, dc, ds;
+    orc_sin_cos_acc(a, &oc, &os);
+    det::sin_cos_rint(a, &dc, &ds);
+    if (oc != dc || os != ds) { bad++; if (bad < 5) printf("  sin_cos_rint a=%lld\n", (long long)a); }
+  }
+  report("sin_cos_rint", nsc, bad);
   // softmax_weight at exact half-way quotients and near the 2^61 sum boundary.
   bad = 0;
   long nw = 0;
