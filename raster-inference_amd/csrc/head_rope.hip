@@ -39,11 +39,12 @@ struct Vec<4> {
 // time, V consecutive values per lane and step, E steps; the first rows' loads
 // are on their way while the cosines are computed. A pair of the half layout
 // meets through the rows' LDS copies, an interleaved pair in one lane (V = 4) or
-// through them as well.
-template <int V, int E, int U>
-__global__ __launch_bounds__(256) void k_head_rope(HeadRopeArgs a, uint32_t lanes) {
+// through them as well. WAVE: a wave per row (the rows' pointers are scalar).
+template <int V, int E, int U, bool WAVE>
+__global__ __launch_bounds__(256) void k_head_rope(HeadRopeArgs a, uint32_t lane_group) {
   extern __shared__ __attribute__((aligned(16))) int32_t lds[];  // cosines, sines, U rows per lane group
-  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, waves = blockDim.x >> 6;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), lanes = WAVE ? 64 : lane_group;
   const uint32_t per_wave = 64 / lanes, li = lane % lanes, hd = a.hd, pairs = a.pairs;
   const uint32_t table = (pairs + 3) & ~3u, row_ld = (hd + 3) & ~3u;
   const uint64_t t = blockIdx.x;
@@ -63,7 +64,7 @@ __global__ __launch_bounds__(256) void k_head_rope(HeadRopeArgs a, uint32_t lane
     int32_t x[U][E][V];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const uint32_t r = r0 + u * step + lane / lanes;
+      const uint32_t r = r0 + u * step + (WAVE ? 0 : lane / lanes);
       on[u] = r < a.total;
       uint32_t h = on[u] ? r : 0;
       s[u] = a.set[0];
@@ -93,19 +94,29 @@ __global__ __launch_bounds__(256) void k_head_rope(HeadRopeArgs a, uint32_t lane
       }
       lds_barrier();
     }
+    int64_t ss[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (!(s[u].flags & 1)) continue;
       // (non-negative terms: the saturating sum is the least of the sum and i64::MAX in any order)
-      int64_t ss = 0;
+      ss[u] = 0;
 #pragma unroll
       for (int e = 0; e < E; ++e)
 #pragma unroll
-        for (int v = 0; v < V; ++v) ss = add_sat64_nn(ss, sq_term(x[u][e][v]));
-      if (lanes == 64) ss = wave_sum_sat64(ss);
+        for (int v = 0; v < V; ++v) ss[u] = add_sat64_nn(ss[u], sq_term(x[u][e][v]));
+      if (WAVE) ss[u] = wave_sum_sat64(ss[u]);
       else
-        for (uint32_t off = 1; off < lanes; off <<= 1) ss = add_sat64_nn(ss, __shfl_xor(ss, int(off), 64));
-      const int32_t scale = rms_scale_from_sumsq(ss, hd, a.eps);
+        for (uint32_t off = 1; off < lanes; off <<= 1) ss[u] = add_sat64_nn(ss[u], __shfl_xor(ss[u], int(off), 64));
+    }
+    // (a wave's U rows: lane u finds the scale of row u)
+    int64_t mine = ss[0];
+    if (WAVE)
+#pragma unroll
+      for (int u = 1; u < U; ++u) mine = lane == uint32_t(u) ? ss[u] : mine;
+    const int32_t found = WAVE ? rms_scale_from_sumsq(mine, hd, a.eps) : 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (!(s[u].flags & 1)) continue;
+      const int32_t scale = WAVE ? __builtin_amdgcn_readlane(found, u) : rms_scale_from_sumsq(ss[u], hd, a.eps);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const uint32_t c = V * (li + 64 * e);
@@ -173,7 +184,9 @@ void launch(const HeadRopeArgs& a, hipStream_t s) {
   uint32_t waves = (a.total + per_wave * U - 1) / (per_wave * U);
   waves = std::min(std::max(waves, a.pairs > 64 ? 2u : 1u), 4u);
   const size_t bytes = (2 * ((a.pairs + 3) & ~3u) + waves * per_wave * U * ((a.hd + 3) & ~3u)) * 4;
-  hipLaunchKernelGGL((k_head_rope<V, E, U>), dim3(unsigned(a.rows)), dim3(64 * waves), bytes, s, a, lanes);
+  const dim3 grid(unsigned(a.rows)), block(64 * waves);
+  if (lanes == 64) hipLaunchKernelGGL((k_head_rope<V, E, U, true>), grid, block, bytes, s, a, lanes);
+  else if constexpr (E == 1) hipLaunchKernelGGL((k_head_rope<V, E, U, false>), grid, block, bytes, s, a, lanes);
 }
 
 }  // namespace
