@@ -34,23 +34,33 @@ struct Vec<4> {
   }
 };
 
+// Q16.16 values as the doubles that they are: mul_sat(a, b) for b given as b
+// 2^-16 (products below 2^62, so the rounded quotient is below 2^46).
+__device__ __forceinline__ double clamp32(double v) {
+  return __builtin_fmin(__builtin_fmax(v, -2147483648.0), 2147483647.0);
+}
+__device__ __forceinline__ double mul_q16(double a, double b16) { return clamp32(mul_rint(a, b16)); }
+
 // One workgroup per token: its threads compute the token's cosines and sines
 // once into LDS, then each group of `lanes` lanes takes up to U head rows at a
 // time, V consecutive values per lane and step, E steps; the first rows' loads
 // are on their way while the cosines are computed. A pair of the half layout
 // meets through the rows' LDS copies, an interleaved pair in one lane (V = 4) or
-// through them as well. WAVE: a wave per row (the rows' pointers are scalar).
+// through them as well. WAVE: a wave per row (the rows' pointers are scalar). The
+// products are double multiply-adds (2 instructions and the clamp, against 11 for
+// one of 64-bit integers). Bound by these instructions at many tokens, then by the
+// bytes: 4096 tokens of 8 / 2 heads of 256 in 28 us, 20 at a copy's rate.
 template <int V, int E, int U, bool WAVE>
 __global__ __launch_bounds__(256) void k_head_rope(HeadRopeArgs a, uint32_t lane_group) {
-  extern __shared__ __attribute__((aligned(16))) int32_t lds[];  // cosines, sines, U rows per lane group
+  extern __shared__ __attribute__((aligned(16))) double table[];  // cosines, sines (times 2^-16), U rows per lane group
   const uint32_t tid = threadIdx.x, lane = tid & 63, waves = blockDim.x >> 6;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), lanes = WAVE ? 64 : lane_group;
   const uint32_t per_wave = 64 / lanes, li = lane % lanes, hd = a.hd, pairs = a.pairs;
-  const uint32_t table = (pairs + 3) & ~3u, row_ld = (hd + 3) & ~3u;
+  const uint32_t entries = (pairs + 3) & ~3u, row_ld = (hd + 3) & ~3u;
   const uint64_t t = blockIdx.x;
-  int32_t* cs = lds;
-  int32_t* sn = lds + table;
-  int32_t* row = lds + 2 * table + (wave * per_wave + lane / lanes) * U * row_ld;
+  double* cs = table;
+  double* sn = table + entries;
+  int32_t* row = reinterpret_cast<int32_t*>(table + 2 * entries) + (wave * per_wave + lane / lanes) * U * row_ld;
   const bool meet = !(V == 4 && a.interleaved);  // pairs meet in LDS
   const uint32_t step = waves * per_wave;
   for (uint32_t r0 = wave * per_wave;; r0 += step * U) {
@@ -89,23 +99,43 @@ __global__ __launch_bounds__(256) void k_head_rope(HeadRopeArgs a, uint32_t lane
       for (uint32_t i = tid; i < pairs; i += blockDim.x) {
         int32_t c, sv;
         sin_cos_rint(rope_angle(pos, a.freq[i]), &c, &sv);
-        cs[i] = a.amplitude == kOneAct ? c : mul_sat(c, a.amplitude);
-        sn[i] = a.amplitude == kOneAct ? sv : mul_sat(sv, a.amplitude);
+        cs[i] = (a.amplitude == kOneAct ? c : mul_sat(c, a.amplitude)) * 0x1p-16;
+        sn[i] = (a.amplitude == kOneAct ? sv : mul_sat(sv, a.amplitude)) * 0x1p-16;
       }
       lds_barrier();
     }
-    int64_t ss[U];
+    // sums of squares, saturating: the terms are non-negative, so that is the
+    // least of the sum and i64::MAX in any order, and below 2^26 nothing saturates
+    uint32_t large = 0;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      // (non-negative terms: the saturating sum is the least of the sum and i64::MAX in any order)
-      ss[u] = 0;
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int e = 0; e < E; ++e)
 #pragma unroll
-        for (int v = 0; v < V; ++v) ss[u] = add_sat64_nn(ss[u], sq_term(x[u][e][v]));
-      if (WAVE) ss[u] = wave_sum_sat64(ss[u]);
-      else
-        for (uint32_t off = 1; off < lanes; off <<= 1) ss[u] = add_sat64_nn(ss[u], __shfl_xor(ss[u], int(off), 64));
+        for (int v = 0; v < V; ++v) large |= uint32_t(x[u][e][v] ^ (x[u][e][v] >> 31));
+    int64_t ss[U] = {};
+    if (!__any(large >> 26)) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+          for (int v = 0; v < V; ++v) ss[u] += sq_term(x[u][e][v]);
+        if (WAVE) ss[u] = wave_sum_wrap64(ss[u]);
+        else
+          for (uint32_t off = 1; off < lanes; off <<= 1) ss[u] += __shfl_xor(ss[u], int(off), 64);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+          for (int v = 0; v < V; ++v) ss[u] = add_sat64_nn(ss[u], sq_term(x[u][e][v]));
+        if (WAVE) ss[u] = wave_sum_sat64(ss[u]);
+        else
+          for (uint32_t off = 1; off < lanes; off <<= 1) ss[u] = add_sat64_nn(ss[u], __shfl_xor(ss[u], int(off), 64));
+      }
     }
     // (a wave's U rows: lane u finds the scale of row u)
     int64_t mine = ss[0];
@@ -125,8 +155,9 @@ __global__ __launch_bounds__(256) void k_head_rope(HeadRopeArgs a, uint32_t lane
         if (s[u].gain) Vec<V>::load(s[u].gain + c, g);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          x[u][e][v] = mul_sat(x[u][e][v], scale);
-          if (s[u].gain) x[u][e][v] = mul_sat(x[u][e][v], g[v]);
+          double y = mul_q16(double(x[u][e][v]), double(scale) * 0x1p-16);
+          if (s[u].gain) y = mul_q16(y, double(g[v]) * 0x1p-16);
+          x[u][e][v] = int32_t(y);
         }
       }
     }
@@ -157,8 +188,8 @@ __global__ __launch_bounds__(256) void k_head_rope(HeadRopeArgs a, uint32_t lane
             const uint32_t i = a.interleaved ? c >> 1 : (second ? c - pairs : c);
             const int32_t other =
                 meet ? row[u * row_ld + (a.interleaved ? (c ^ 1) : (second ? c - pairs : c + pairs))] : x[u][e][v ^ (V > 1)];
-            const int32_t p = mul_sat(x[u][e][v], cs[i]), q = mul_sat(other, sn[i]);
-            y[v] = second ? add_sat(p, q) : sub_sat(p, q);
+            const double p = mul_q16(double(x[u][e][v]), cs[i]), q = mul_q16(double(other), sn[i]);
+            y[v] = int32_t(clamp32(second ? p + q : p - q));
           }
 #pragma unroll
           for (int v = 0; v < V; ++v) x[u][e][v] = y[v];
@@ -183,7 +214,7 @@ void launch(const HeadRopeArgs& a, hipStream_t s) {
   const uint32_t per_wave = 64 / lanes;
   uint32_t waves = (a.total + per_wave * U - 1) / (per_wave * U);
   waves = std::min(std::max(waves, a.pairs > 64 ? 2u : 1u), 4u);
-  const size_t bytes = (2 * ((a.pairs + 3) & ~3u) + waves * per_wave * U * ((a.hd + 3) & ~3u)) * 4;
+  const size_t bytes = (4 * ((a.pairs + 3) & ~3u) + waves * per_wave * U * ((a.hd + 3) & ~3u)) * 4;
   const dim3 grid(unsigned(a.rows)), block(64 * waves);
   if (lanes == 64) hipLaunchKernelGGL((k_head_rope<V, E, U, true>), grid, block, bytes, s, a, lanes);
   else if constexpr (E == 1) hipLaunchKernelGGL((k_head_rope<V, E, U, false>), grid, block, bytes, s, a, lanes);
