@@ -227,12 +227,17 @@ __device__ __forceinline__ void score_tile(const v4i (&k)[NSUB][3], const v4i* q
 
 // Scores: a block takes up to 64 query rows (digits in LDS, converted once) and
 // the keys of one chunk, 16 per wave and step, which each wave loads and takes
-// apart in registers: no wave waits for another between its tiles.
-template <int NSUB, int MODE>
-__global__ __launch_bounds__(kThreads, NSUB <= 4 ? 4 : 2) void k_tree_scores(Launch p) {
+// apart in registers: no wave waits for another between its tiles. AHEAD: up to
+// 128 rows, half the waves, each step's keys loaded during the step before. At
+// 4096 rows of 8256 keys of 256 dims (16 sets of 256 rows) that takes 104 us
+// against 122 (the device copies its 330 MB, of which the scores are 135, in 67);
+// fewer than 65 rows leave the loads to twice the waves.
+template <int NSUB, int MODE, bool AHEAD>
+__global__ __launch_bounds__(kThreads, NSUB <= 4 && !AHEAD ? 4 : 2) void k_tree_scores(Launch p) {
   extern __shared__ __attribute__((aligned(16))) int8_t lds[];  // [query tile][substep][digit][lane]
-  __shared__ int32_t rmax[64];  // each row's largest score so far
-  __shared__ Sight sight[64];
+  constexpr uint32_t kRows = AHEAD ? 128 : 64;
+  __shared__ int32_t rmax[kRows];  // each row's largest score so far
+  __shared__ Sight sight[kRows];
   __shared__ uint32_t qwide, last_start;
   const Item it = item_of(p, p.chunks, p.row_blocks);
   if (!it.on) return;
@@ -245,10 +250,15 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 ? 4 : 2) void k_tree_scores(Lau
   const uint32_t tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = l & 15, g = l >> 4;
   const uint32_t kvh = p.kv0 + it.kvh, hd = a.hd;
   if (tid < 64) {
-    const Sight v = sight_of(a, s, min(r0 + tid, R - 1) / a.groups);
-    const uint32_t m = uint32_t(wave_max64(int64_t(v.start)));
-    sight[tid] = v;
-    rmax[tid] = INT32_MIN;
+    uint32_t m = 0;
+#pragma unroll
+    for (uint32_t r = tid; r < kRows; r += 64) {
+      const Sight v = sight_of(a, s, min(r0 + r, R - 1) / a.groups);
+      m = max(m, v.start);
+      sight[r] = v;
+      rmax[r] = INT32_MIN;
+    }
+    m = uint32_t(wave_max64(int64_t(m)));
     if (tid == 0) qwide = 0, last_start = m;
   }
   __syncthreads();
@@ -304,10 +314,9 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 ? 4 : 2) void k_tree_scores(Lau
     atomicMax(&rmax[16 * T + i], m);
   };
   uint64_t later0 = 0, later1 = 0;  // key tiles that are not narrow (at most 128 per wave and chunk; wave-uniform)
-  for (uint32_t key0 = k0 + 16 * wave, t = 0; key0 < k1; key0 += 16 * kWaves, ++t) {
+  int32_t x[NSUB][4][4];
+  auto load_k = [&](uint32_t key0) {
     const int32_t* src = row_ptr(s, s.k, a.k, a.kv_ld, key0 + i, off);
-    v4i k3[NSUB][3];
-    int32_t x[NSUB][4][4];
     uint32_t hdl = hd;
     if (MODE != kWhole) asm volatile("" : "+s"(hdl));  // (offsets kept over the loop would spill)
 #pragma unroll
@@ -319,6 +328,11 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 ? 4 : 2) void k_tree_scores(Lau
         else load4<MODE>(src, 64 * sub + 16 * j + 4 * g, hdl, x[sub][j]);
         if (MODE == kScalar) __builtin_amdgcn_sched_barrier(0);  // (addresses of four values at a time)
       }
+  };
+  if (AHEAD && k0 + 16 * wave < k1) load_k(k0 + 16 * wave);
+  for (uint32_t key0 = k0 + 16 * wave, t = 0; key0 < k1; key0 += 16 * kWaves, ++t) {
+    v4i k3[NSUB][3];
+    if (!AHEAD) load_k(key0);
     uint32_t all = 0;
 #pragma unroll
     for (int sub = 0; sub < NSUB; ++sub)
@@ -334,6 +348,7 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 ? 4 : 2) void k_tree_scores(Lau
     for (int sub = 0; sub < NSUB; ++sub)
 #pragma unroll
       for (int q = 0; q < 3; ++q) asm volatile("" : "+v"(k3[sub][q]));
+    if (AHEAD && key0 + 16 * kWaves < k1) load_k(key0 + 16 * kWaves);
     if (qw || __any(all != 0)) {
       if (t < 64) later0 |= 1ull << t;
       else later1 |= 1ull << (t - 64);
@@ -964,12 +979,12 @@ uint64_t plan(const TreeArgs& a, const TreeSeq* seqs, const Group& g, Launch& p)
   }
   p.wide_k = w4;
   p.wide_v = w2;
-  // 64 query rows per block; 32 where their digits or their sums' registers would
-  // leave the device half empty
-  p.block_rows = std::min<uint32_t>(uint32_t(up(most, 16)), a.hd <= 256 ? 64 : 32);
+  // 64 query rows per block, 128 with loads a step ahead; 32 where their digits or
+  // their sums' registers would leave the device half empty
+  p.block_rows = std::min<uint32_t>(uint32_t(up(most, 16)), a.hd <= 256 ? (most > 64 && w4 ? 128 : 64) : 32);
   p.row_blocks = (most + p.block_rows - 1) / p.block_rows;
   units = uint64_t(p.n_seq) * g.nkv * p.row_blocks;
-  p.chunk = chunk_of(keys, units, 512, 16 * kWaves);
+  p.chunk = chunk_of(keys, units, p.block_rows > 64 ? 256 : 512, 16 * kWaves);
   p.chunks = uint32_t((keys + p.chunk - 1) / p.chunk);
   p.whole = keys <= kRowKeys && (p.rows >= 256 || keys <= 4096);
   p.groups = a.hd <= 32 ? 1 : a.hd <= 64 ? 2 : a.hd <= 128 ? 4 : 8;
@@ -1004,9 +1019,15 @@ void launch_scores(const Launch& p, uint32_t blocks, hipStream_t s) {
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 128 << 10);
     hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), lds, s, p);
   };
-  if (!p.wide_k) go(&k_tree_scores<NSUB, kScalar>);
-  else if (p.a.hd == 64 * NSUB) go(&k_tree_scores<NSUB, kWhole>);
-  else go(&k_tree_scores<NSUB, kVec4>);
+  if constexpr (NSUB <= 4)
+    if (p.block_rows > 64) {
+      if (p.a.hd == 64 * NSUB) go(&k_tree_scores<NSUB, kWhole, true>);
+      else go(&k_tree_scores<NSUB, kVec4, true>);
+      return;
+    }
+  if (!p.wide_k) go(&k_tree_scores<NSUB, kScalar, false>);
+  else if (p.a.hd == 64 * NSUB) go(&k_tree_scores<NSUB, kWhole, false>);
+  else go(&k_tree_scores<NSUB, kVec4, false>);
 }
 template <int RT>
 void launch_wsum(const Launch& p, uint32_t blocks, hipStream_t s) {
