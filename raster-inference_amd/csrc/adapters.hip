@@ -33,7 +33,6 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 constexpr uint32_t kOp = 1024;       // one MFMA operand: 64 lanes x 16 bytes
 constexpr uint32_t kNoRow = ~0u;
 constexpr uint32_t kSmallRows = 64;  // rows whose tiles every workgroup finds itself
-constexpr uint32_t kUpTiles = 16;    // 16-row tiles of B per workgroup
 constexpr uint32_t kStepCols = 256;  // columns per step of A x
 
 struct Plan {
@@ -41,6 +40,7 @@ struct Plan {
   uint32_t tiles;      // most tiles
   uint32_t chunk, chunks;  // steps of kStepCols per chunk of K
   uint32_t ranks;      // values per row of the partial sums (max_rank)
+  uint32_t up_tiles;   // 16-row tiles of B per workgroup of B h
   int vec;             // 16-byte aligned activation rows
   int out4;            // 16-byte aligned output rows
   int64_t* planes;     // [chunk][16 tile + row][ranks]
@@ -175,6 +175,21 @@ __device__ __forceinline__ int64_t total(const v4i (&acc)[8], int r) {
   return int64_t(y);
 }
 
+// requant(sum times by) of one component where the digits j have 0 .. 2 only, as
+// the whole double that it is: sums below 2^52 times scales are one rounded
+// multiply-add (the products of the integer form stay below 2^62, so that nothing
+// has wrapped there either). 8 instructions against 40.
+template <int P>
+__device__ __forceinline__ double scaled(const v4i (&acc)[8], int r, int32_t by, bool& far) {
+  // (at most 256 columns of 128 x 128 per pair, four pairs: words of two sums are below 2^32 / 2)
+  double y = double(acc[0][r] + (acc[1][r] << 8));
+  y = __builtin_fma(double(P > 1 ? acc[2][r] + (acc[3][r] << 8) : acc[2][r]), 65536.0, y);
+  if (P > 2) y = __builtin_fma(double(acc[4][r] + (acc[5][r] << 8)), 4294967296.0, y);
+  const double b = double(by);
+  far = far || !(__builtin_fabs(y) < 4503599627370496.0) || !(__builtin_fabs(y * b) < 4611686018427387904.0);
+  return mul_rint(y, b * 0x1p-16);
+}
+
 // A x of one tile, one chunk of K and up to 64 rank rows. Per step of 256
 // columns each wave takes its 64 columns of the rows apart into LDS (the
 // weights' tile-steps: half h of step s, lane 16 g + i, holds columns 128 s +
@@ -264,67 +279,22 @@ __global__ __launch_bounds__(256) void k_adapter_down(Plan p) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) y[r] = int64_t(uint64_t(y[r]) + uint64_t(share[(w * 4 + r) * 64 + l]));
   }
-  if (!on) return;
+  if (!on || t.row[l & 15] == kNoRow) return;
   int64_t* o = p.planes + ((uint64_t(blockIdx.y) * p.tiles + blockIdx.x) * 16 + (l & 15)) * p.ranks + 16 * rank_tile +
                4 * (l >> 4);
 #pragma unroll
   for (int r = 0; r < 4; ++r) o[r] = y[r];
 }
 
-// B h of one tile and kUpTiles 16-row tiles of B.
-template <int P>
-__device__ __forceinline__ void up_tiles(const Plan& p, const DevAdapter& ad, const Tile& t, const v4i* digits, bool wide) {
-  const uint32_t l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = l & 15, g = l >> 4;
-  const uint32_t subs = (ad.kg + 3) / 4, row = t.row[i];
-  const uint64_t tiles = (p.a.rows + 15) / 16, t0 = uint64_t(blockIdx.y) * kUpTiles;
-  for (uint64_t T = t0 + wave; T < min(t0 + kUpTiles, tiles); T += 4) {
-    v4i acc[8];
-#pragma unroll
-    for (int s = 0; s < 8; ++s) acc[s] = v4i{0, 0, 0, 0};
-    for (uint32_t s = 0; s < subs; ++s) {
-      v4i w[P];
-#pragma unroll
-      for (int q = 0; q < P; ++q)
-        w[q] = 4 * s + g < ad.kg
-                   ? *reinterpret_cast<const v4i*>(ad.b + ((T * P + q) * ad.kg + 4 * s + g) * 256 + i * 16)
-                   : v4i{0, 0, 0, 0};
-      multiply<P>(w, digits + s * 5 * 64, l, wide, acc);
-    }
-    // lane l, component r: output 16 T + 4 g + r of row i
-    const uint64_t n = 16 * T + 4 * g;
-    if (row == kNoRow || n >= p.a.rows) continue;
-    int32_t* o = p.a.out + uint64_t(row) * p.a.rows + n;
-    int32_t y[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r)  // (b_scale holds whole tiles)
-      y[r] = mul_sat(requant(int64_t(uint64_t(total(acc, r)) * uint64_t(int64_t(ad.b_scale[n + r])))), ad.scale);
-    if (p.out4) {
-      int4 v = *reinterpret_cast<const int4*>(o);
-      v.x = add_sat(v.x, y[0]), v.y = add_sat(v.y, y[1]), v.z = add_sat(v.z, y[2]), v.w = add_sat(v.w, y[3]);
-      *reinterpret_cast<int4*>(o) = v;
-    } else {
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (n + r < p.a.rows) o[r] = add_sat(o[r], y[r]);
-    }
-  }
-}
-__global__ __launch_bounds__(256) void k_adapter_up(Plan p) {
-  extern __shared__ __attribute__((aligned(16))) int8_t lds[];  // digits of h: [64 rank rows][digit][lane], then h
-  __shared__ uint32_t wide;
-  __shared__ Tile t;
-  const uint32_t tid = threadIdx.x;
-  if (tid == 0) wide = 0;
-  find_tile(p, blockIdx.x, t);
-  if (t.adapter == kNoRow) return;
-  const DevAdapter ad = p.a.set[t.adapter];
-  const uint32_t subs = (ad.kg + 3) / 4, ranks = 64 * subs;
-  // h: the chunks' sums, a value per thread
+// h of one tile: its chunks' sums, a value per thread, then their digits, 16
+// values per thread (one operand lane).
+__device__ __forceinline__ void rank_rows(const Plan& p, const DevAdapter& ad, const Tile& t, int8_t* lds, uint32_t* wide) {
+  const uint32_t tid = threadIdx.x, subs = (ad.kg + 3) / 4, ranks = 64 * subs;
   int32_t* hs = reinterpret_cast<int32_t*>(lds + subs * 5 * kOp);  // [row][ranks]
   for (uint32_t u = tid; u < 16 * 16 * ad.kg; u += 256) {
     const uint32_t i = u / (16 * ad.kg), k = u % (16 * ad.kg);
     int32_t h = 0;
-    if (k < ad.rank) {
+    if (k < ad.rank && t.row[i] != kNoRow) {
       const int64_t* src = p.planes + (uint64_t(blockIdx.x) * 16 + i) * p.ranks + k;
       const uint64_t ld = uint64_t(p.tiles) * 16 * p.ranks;
       uint64_t y = 0;
@@ -341,8 +311,7 @@ __global__ __launch_bounds__(256) void k_adapter_up(Plan p) {
     }
     hs[i * ranks + k] = h;
   }
-  __syncthreads();
-  // its digits: 16 values per thread, one operand lane
+  lds_barrier();
   for (uint32_t u = tid; u < subs * 64; u += 256) {
     const int4* src = reinterpret_cast<const int4*>(hs + (u & 15) * ranks + 16 * (u >> 4));
     int32_t h[16];
@@ -352,16 +321,88 @@ __global__ __launch_bounds__(256) void k_adapter_up(Plan p) {
       h[4 * q] = v.x, h[4 * q + 1] = v.y, h[4 * q + 2] = v.z, h[4 * q + 3] = v.w;
     }
     v4i d[5];
-    if (digits16(h, d)) wide = 1;
+    if (digits16(h, d)) *wide = 1;
     v4i* dst = reinterpret_cast<v4i*>(lds) + (u >> 6) * 5 * 64 + (u & 63);
 #pragma unroll
     for (int j = 0; j < 5; ++j) dst[j * 64] = d[j];
   }
-  __syncthreads();
+  lds_barrier();
+}
+// B h of one tile and p.up_tiles 16-row tiles of B, round the four waves. What
+// the first 64 rank rows take from memory is loaded a tile ahead, for the first
+// tile while h is made.
+template <int P>
+__device__ __forceinline__ void up_tiles(const Plan& p, const DevAdapter& ad, const Tile& t, int8_t* lds, uint32_t* wide_h) {
+  const uint32_t l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = l & 15, g = l >> 4;
+  const uint32_t subs = (ad.kg + 3) / 4, row = t.row[i];
+  const uint64_t tiles = (p.a.rows + 15) / 16, end = min(uint64_t(blockIdx.y + 1) * p.up_tiles, tiles);
+  int32_t* out = p.a.out + uint64_t(row == kNoRow ? 0 : row) * p.a.rows;
+  auto weights = [&](uint64_t T, uint32_t s, v4i (&w)[P]) {
+#pragma unroll
+    for (int q = 0; q < P; ++q)
+      w[q] = 4 * s + g < ad.kg ? *reinterpret_cast<const v4i*>(ad.b + ((T * P + q) * ad.kg + 4 * s + g) * 256 + i * 16)
+                               : v4i{0, 0, 0, 0};
+  };
+  v4i w[P];
+  int4 scale, old;
+  auto load = [&](uint64_t T) {  // lane l, component r: output 16 T + 4 g + r of row i
+    const uint64_t n = 16 * T + 4 * g;
+    weights(T, 0, w);
+    scale = *reinterpret_cast<const int4*>(ad.b_scale + n);  // (b_scale holds whole tiles)
+    if (p.out4 && row != kNoRow && n < p.a.rows) old = *reinterpret_cast<const int4*>(out + n);
+  };
+  uint64_t T = uint64_t(blockIdx.y) * p.up_tiles + wave;
+  if (T < end) load(T);
+  rank_rows(p, ad, t, lds, wide_h);
   const v4i* digits = reinterpret_cast<const v4i*>(lds);
-  if (ad.b_planes == 1) up_tiles<1>(p, ad, t, digits, wide != 0);
-  else if (ad.b_planes == 2) up_tiles<2>(p, ad, t, digits, wide != 0);
-  else up_tiles<4>(p, ad, t, digits, wide != 0);
+  const bool wide = *wide_h != 0;
+  const double by_all = double(ad.scale) * 0x1p-16;
+#pragma unroll 1
+  for (; T < end; T += 4) {
+    v4i acc[8];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) acc[s] = v4i{0, 0, 0, 0};
+    uint32_t s = 0;
+    do {
+      if (s) weights(T, s, w);
+      multiply<P>(w, digits + s * 5 * 64, l, wide, acc);
+    } while (++s < subs);
+    const int32_t by[4] = {scale.x, scale.y, scale.z, scale.w}, was[4] = {old.x, old.y, old.z, old.w};
+    if (T + 4 < end) load(T + 4);
+    const uint64_t n = 16 * T + 4 * g;
+    if (row == kNoRow || n >= p.a.rows) continue;
+    int32_t y[4];
+    bool far = wide;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) y[r] = to_i32(mul_rint(double(to_i32(scaled<P>(acc, r, by[r], far))), by_all));
+    if (__any(far)) {
+#pragma unroll
+      for (int s = 0; s < 8; ++s) asm volatile("" : "+v"(acc[s]));  // (a branch in earnest)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        y[r] = mul_sat(requant(int64_t(uint64_t(total(acc, r)) * uint64_t(int64_t(by[r])))), ad.scale);
+    }
+    if (p.out4) {
+      *reinterpret_cast<int4*>(out + n) =
+          make_int4(add_sat(was[0], y[0]), add_sat(was[1], y[1]), add_sat(was[2], y[2]), add_sat(was[3], y[3]));
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (n + r < p.a.rows) out[n + r] = add_sat(out[n + r], y[r]);
+    }
+  }
+}
+__global__ __launch_bounds__(256) void k_adapter_up(Plan p) {
+  extern __shared__ __attribute__((aligned(16))) int8_t lds[];  // digits of h: [64 rank rows][digit][lane], then h
+  __shared__ uint32_t wide;
+  __shared__ Tile t;
+  if (threadIdx.x == 0) wide = 0;
+  find_tile(p, blockIdx.x, t);
+  if (t.adapter == kNoRow) return;
+  const DevAdapter ad = p.a.set[t.adapter];
+  if (ad.b_planes == 1) up_tiles<1>(p, ad, t, lds, &wide);
+  else if (ad.b_planes == 2) up_tiles<2>(p, ad, t, lds, &wide);
+  else up_tiles<4>(p, ad, t, lds, &wide);
 }
 
 uint64_t up(uint64_t v, uint64_t a) { return (v + a - 1) / a * a; }
@@ -377,6 +418,10 @@ uint64_t plan(const AdapterArgs& a, Plan& p) {
   const uint64_t full = (a.m + 15) / 16 * ((a.max_rank + 63) / 64);
   p.chunk = uint32_t(std::min<uint64_t>(std::max<uint64_t>(full * steps / 512, 1), 8192 / kStepCols));
   p.chunks = (steps + p.chunk - 1) / p.chunk;
+  // of B's tiles one per wave, up to 16 of them as soon as three workgroups per
+  // CU are left (h is made by every one)
+  p.up_tiles = 4;
+  while (p.up_tiles < 16 && uint64_t(p.tiles) * ((a.rows + 15) / 16) / p.up_tiles > 768) p.up_tiles *= 2;
   p.vec = a.cols % 4 == 0 && reinterpret_cast<uintptr_t>(a.act) % 16 == 0;
   p.out4 = a.rows % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
   uint64_t at = 0;
@@ -423,7 +468,7 @@ void launch_adapters(const AdapterArgs& a, void* work, hipStream_t s) {
     const unsigned rank_groups = (a.max_rank + 63) / 64;
     if (p.a.m > kSmallRows) hipLaunchKernelGGL(k_adapter_sort, dim3(1), dim3(kSortThreads), 0, s, p);
     hipLaunchKernelGGL(k_adapter_down, dim3(p.tiles, p.chunks, rank_groups), dim3(256), 0, s, p);
-    hipLaunchKernelGGL(k_adapter_up, dim3(p.tiles, unsigned((a.rows + 16 * kUpTiles - 1) / (16 * kUpTiles))), dim3(256),
+    hipLaunchKernelGGL(k_adapter_up, dim3(p.tiles, unsigned((a.rows + 16 * p.up_tiles - 1) / (16 * p.up_tiles))), dim3(256),
                        rank_groups * (5 + 4) * kOp, s, p);
   }
 }

@@ -34,13 +34,6 @@ struct Vec<4> {
   }
 };
 
-// Nearest i32 of a whole double, the ends for what lies beyond them: what the
-// conversion instruction does (a C++ conversion leaves it open).
-__device__ __forceinline__ int32_t to_i32(double v) {
-  int32_t r;
-  asm("v_cvt_i32_f64 %0, %1" : "=v"(r) : "v"(v));
-  return r;
-}
 // round(a b 2^16) 2^-16 for |a b| below 2^35 (mul_rint at a unit of 2^-16).
 __device__ __forceinline__ double mul_rint16(double a, double b) {
   constexpr double kWhole = 103079215104.0;  // 1.5 2^36

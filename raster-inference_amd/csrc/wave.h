@@ -68,6 +68,13 @@ __device__ __forceinline__ uint64_t readlane64(uint64_t v, int lane) {
   return (uint64_t(hi) << 32) | lo;
 }
 
+// Nearest i32 of a whole double, the ends for what lies beyond them: what the
+// conversion instruction does (a C++ conversion leaves it open).
+__device__ __forceinline__ int32_t to_i32(double v) {
+  int32_t r;
+  asm("v_cvt_i32_f64 %0, %1" : "=v"(r) : "v"(v));
+  return r;
+}
 struct OpWrapAdd {
   __device__ __forceinline__ uint64_t operator()(uint64_t a, uint64_t b) const { return a + b; }
 };
