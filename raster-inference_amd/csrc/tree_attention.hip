@@ -455,16 +455,15 @@ __global__ __launch_bounds__(256) void k_tree_terms(Launch p) {
       if (!plain) in = in && sees(v, s.rows, k);
       double e = 0;
       if (__any(in)) {
-        e = in ? softmax_term(gap) : 0.0;
+        e = softmax_term_or_zero(gap, in);
         if (in && gap == 0) first = min(first, k);
         sum += e;
       }
       // (2^32 in 32 bits: all ones, which no other term is)
-      if (k < k2) sc[k] = int32_t(uint32_t(__builtin_fmin(e, 4294967295.0)));
+      if (k < k2) sc[k] = int32_t(to_u32(e));
     }
   }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
+  sum = double(wave_sum_wrap64(int64_t(sum)));
   first = ~uint32_t(wave_max64(int64_t(~first)));
   if (l == 0) {
     p.psum[uint64_t(id) * p.chunks + chunk] = int64_t(sum);
@@ -496,10 +495,10 @@ __device__ inline Recip recip_of(int64_t sum) {
   }
   return r;
 }
-__device__ __forceinline__ uint32_t weight_of(uint32_t e, uint32_t m, uint32_t sh, bool& unsure) {
+__device__ __forceinline__ uint32_t weight_of(uint32_t e, uint32_t m, uint32_t sh, uint32_t& margin) {
   const uint32_t half = 1u << (sh - 1), near = 1u << (sh - 13);
-  const uint32_t y = __umulhi(e, m) + half, f = y & (2 * half - 1);
-  unsure = f - near >= 2 * half - 2 * near;
+  const uint32_t y = __umulhi(e, m) + half;
+  margin = (y & (2 * half - 1)) - near;  // from 2 half - 2 near on: next to a border
   return y >> sh;
 }
 
@@ -507,13 +506,13 @@ __device__ __forceinline__ uint32_t weight_of(uint32_t e, uint32_t m, uint32_t s
 // 0x8080), a word each, their sum; keys of weights above 32639 go to `end` (their
 // digits are those of w - 65536).
 __device__ __forceinline__ uint2 weights4(const uint32_t (&e)[4], const Recip& rc, uint32_t key, int32_t& total, RowEnd* end) {
-  uint32_t w[4], unsure = 0;
+  uint32_t w[4], margin[4], unsure = 0;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    bool no;
-    w[q] = weight_of(e[q], rc.m, rc.sh, no);
-    unsure |= uint32_t(no) << q;
-  }
+  for (int q = 0; q < 4; ++q) w[q] = weight_of(e[q], rc.m, rc.sh, margin[q]);
+  const uint32_t border = (1u << rc.sh) - (2u << (rc.sh - 13));
+  if (max(max(margin[0], margin[1]), max(margin[2], margin[3])) >= border)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) unsure |= uint32_t(margin[q] >= border) << q;
 #pragma unroll 1
   for (; unsure; unsure &= unsure - 1) {
     const int at = __builtin_ctz(unsure);
@@ -596,17 +595,18 @@ __global__ __launch_bounds__(256) void k_tree_rows(Launch p, uint32_t lds_row) {
       const bool seen = gap < (1u << 20) && ((vis >> q) & 1u);
       double y = 0;
       if (__any(seen)) {
-        y = softmax_term(seen ? gap : (1u << 20) - 1);
-        y = seen ? y : 0.0;
-        if (seen && gap == 0) first = min(first, k + q);
+        y = softmax_term_or_zero(gap, seen);
+        if (__any(gap == 0)) {
+          asm volatile("");
+          if (seen && gap == 0) first = min(first, k + q);
+        }
         sum += y;
       }
-      e[q] = uint32_t(__builtin_fmin(y, 4294967295.0));  // (2^32: all ones, which no other term is)
+      e[q] = to_u32(y);  // (2^32: all ones, which no other term is)
     }
     *reinterpret_cast<uint4*>(terms + k) = make_uint4(e[0], e[1], e[2], e[3]);
   }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
+  sum = double(wave_sum_wrap64(int64_t(sum)));
   first = ~uint32_t(wave_max64(int64_t(~first)));
   if (l == 0) red_sum[wave] = sum, red_first[wave] = first;
   __syncthreads();
@@ -624,8 +624,7 @@ __global__ __launch_bounds__(256) void k_tree_rows(Launch p, uint32_t lds_row) {
     const uint2 w = weights4(e, rc, k, total, &ends[in]);
     if (on) put4(reinterpret_cast<int8_t*>(sc), k, w);
   }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o, 64);
+  total = int32_t(wave_sum_wrap64(total));
   if (l == 0) red_total[wave] = total;
   __syncthreads();
   if (lane == 0 && on) {
@@ -656,8 +655,7 @@ __global__ __launch_bounds__(256) void k_tree_weights(Launch p) {
     const uint32_t e[4] = {t.x, t.y, t.z, t.w};
     put4(p.weights + 2 * row, k, weights4(e, rc, k, total, &p.ends[id]));
   }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o, 64);
+  total = int32_t(wave_sum_wrap64(total));
   if (l == 0) p.pweight[uint64_t(id) * p.chunks + chunk] = total;
 }
 

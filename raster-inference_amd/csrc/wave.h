@@ -75,6 +75,13 @@ __device__ __forceinline__ int32_t to_i32(double v) {
   asm("v_cvt_i32_f64 %0, %1" : "=v"(r) : "v"(v));
   return r;
 }
+// The same for u32 (2^32 and above: all ones).
+__device__ __forceinline__ uint32_t to_u32(double v) {
+  uint32_t r;
+  asm("v_cvt_u32_f64 %0, %1" : "=v"(r) : "v"(v));
+  return r;
+}
+
 struct OpWrapAdd {
   __device__ __forceinline__ uint64_t operator()(uint64_t a, uint64_t b) const { return a + b; }
 };
