@@ -124,16 +124,35 @@ __device__ inline Sight sight_of(const TreeArgs& a, const Seq& s, uint32_t draft
 __device__ inline bool sees(const Sight& v, uint32_t rows, uint32_t key) {
   return key < rows ? key >= v.start : (key - rows < 64 && ((v.mask >> (key - rows)) & 1));
 }
-// Row `key` of the cached rows followed by the drafted ones (this kv head's
-// values); keys past them give the last drafted row.
-__device__ inline const int32_t* row_ptr(const Seq& s, const int32_t* cache, const int32_t* drafted, uint64_t kv_ld,
-                                         uint32_t key, uint64_t off) {
-  uint64_t p = s.first + key;
-  if (s.wrap && p >= s.wrap) p -= s.wrap;
-  const bool cached = key < s.rows;
-  const uint64_t d = s.row0 + min(key - s.rows, s.drafts - 1);
-  return (cached ? cache : drafted) + (cached ? p * s.ld : d * kv_ld) + off;
-}
+// The cached rows of a sequence followed by its drafted ones, one kv head's
+// values. Held in registers: read from the arguments in each lane's branch they
+// would cost a round trip to memory per row.
+struct Rows {
+  const int32_t* cache;
+  const int32_t* drafted;  // its first drafted row
+  uint64_t ld, kv_ld, first, wrap;
+  uint32_t rows, drafts;
+  __device__ __forceinline__ Rows(const Seq& s, const int32_t* c, const int32_t* d, uint64_t kv, uint64_t off) {
+    const int32_t *c0 = c + off, *d0 = d + s.row0 * kv + off;
+    uint64_t l0 = s.ld, f0 = s.first, w0 = s.wrap;
+    uint32_t r0 = s.rows, n0 = s.drafts;
+    asm volatile("" : "+s"(c0), "+s"(d0), "+s"(l0), "+s"(kv));
+    asm volatile("" : "+s"(f0), "+s"(w0), "+s"(r0), "+s"(n0));
+    cache = c0, drafted = d0, ld = l0, kv_ld = kv, first = f0, wrap = w0, rows = r0, drafts = n0;
+  }
+  // Row `key`; keys past them give the last drafted row.
+  __device__ __forceinline__ const int32_t* at(uint32_t key) const {
+    uint64_t p = first + key;
+    p -= wrap && p >= wrap ? wrap : 0;
+    // (values here: a choice between the members would become one of their addresses)
+    const int32_t *c = cache, *d = drafted;
+    uint64_t cl = ld, dl = kv_ld;
+    asm("" : "+s"(c), "+s"(d), "+s"(cl), "+s"(dl));
+    const bool cached = key < rows;
+    const uint64_t row = cached ? p : uint64_t(min(key - rows, drafts - 1));
+    return (cached ? c : d) + row * (cached ? cl : dl);
+  }
+};
 
 // Digits of four values: word j holds digit j of each; `all` collects the words.
 __device__ __forceinline__ void digits4(const int32_t (&x)[4], uint32_t (&w)[4], uint32_t& all) {
@@ -296,6 +315,7 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 && !AHEAD ? 4 : 2) void k_tree_
   const uint32_t id0 = s.id0 + it.kvh * R + r0;
   int32_t* sc = p.scores + s.score0 + uint64_t(it.kvh * R + r0) * s.score_ld;
   const uint64_t off = uint64_t(kvh) * hd;
+  const Rows keys(s, s.k, a.k, a.kv_ld, off);
   const uint32_t seen_from = __builtin_amdgcn_readfirstlane(last_start);
   // scores of tile T and the keys from key0 on: stored, and the largest seen one kept
   auto finish = [&](uint32_t T, uint32_t key0, const int32_t (&out)[4]) {
@@ -316,7 +336,7 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 && !AHEAD ? 4 : 2) void k_tree_
   uint64_t later0 = 0, later1 = 0;  // key tiles that are not narrow (at most 128 per wave and chunk; wave-uniform)
   int32_t x[NSUB][4][4];
   auto load_k = [&](uint32_t key0) {
-    const int32_t* src = row_ptr(s, s.k, a.k, a.kv_ld, key0 + i, off);
+    const int32_t* src = keys.at(key0 + i);
     uint32_t hdl = hd;
     if (MODE != kWhole) asm volatile("" : "+s"(hdl));  // (offsets kept over the loop would spill)
 #pragma unroll
@@ -368,7 +388,7 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 && !AHEAD ? 4 : 2) void k_tree_
   for (uint32_t h = 0; h < 2; ++h)
     for (uint64_t bits = h ? later1 : later0; bits; bits &= bits - 1) {
       const uint32_t key0 = k0 + 16 * wave + 16 * kWaves * (64 * h + uint32_t(__builtin_ctzll(bits)));
-      const int32_t* src = row_ptr(s, s.k, a.k, a.kv_ld, key0 + i, off);
+      const int32_t* src = keys.at(key0 + i);
 #pragma unroll 1
       for (uint32_t T = 0; T < tiles; ++T) {
         const int32_t* qsrc = q_row(T);
@@ -687,6 +707,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_tree_wsum(Launch p) {
   const bool on = split < splits && dim0 < hd && k0 < k1;
   const uint32_t rows = min(R - r0, p.sum_rows), id0 = s.id0 + it.kvh * R + r0;
   const uint64_t off = uint64_t(kvh) * hd;
+  const Rows values(s, s.v, a.v, a.kv_ld, off);
   const uint32_t dim = dim0 + 2 * i, dim_in = dim + 1 < hd ? dim : (hd > 1 ? hd - 2 : 0);  // (sums of dims past hd are dropped)
   const uint32_t run_off = 16 * g * uint32_t(s.ld) + dim_in;
   auto load_v = [&](uint32_t k, int32_t (&x)[16][2]) {
@@ -706,10 +727,16 @@ __global__ __launch_bounds__(kThreads, 2) void k_tree_wsum(Launch p) {
     // (weights are zero from the row's end on)
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const int32_t* row = row_ptr(s, s.v, a.v, a.kv_ld, min(k + 16 * g + e, n - 1), off);
-      x[e][0] = to_global(row)[min(dim, hd - 1)];
-      x[e][1] = to_global(row)[min(dim + 1, hd - 1)];
-      __builtin_amdgcn_sched_barrier(0);  // (one row's address at a time)
+      const int32_t* row = values.at(min(k + 16 * g + e, n - 1));
+      if (p.wide_v) {
+        typedef int v2 __attribute__((ext_vector_type(2)));
+        const v2 t = *(global_ptr<const v2>)(to_global(row) + dim_in);
+        x[e][0] = t.x, x[e][1] = t.y;
+      } else {
+        x[e][0] = to_global(row)[min(dim, hd - 1)];
+        x[e][1] = to_global(row)[min(dim + 1, hd - 1)];
+      }
+      if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (four rows' addresses at a time)
     }
   };
   // this lane's pieces of the digits of step `st`: slot c of a split's 2 RT has rows 8 c ..
@@ -882,7 +909,8 @@ __global__ __launch_bounds__(256) void k_tree_join(Launch p) {
   }
   int32_t* out = a.out + (s.row0 + row / a.groups) * a.out_ld + uint64_t(kvh * a.groups + row % a.groups) * a.hd;
   const uint64_t off = uint64_t(kvh) * a.hd;
-  const int32_t* v = row_ptr(s, s.v, a.v, a.kv_ld, end.first == kNone ? n - 1 : end.first, off);
+  const Rows values(s, s.v, a.v, a.kv_ld, off);
+  const int32_t* v = values.at(min(end.first, n - 1));
   const uint32_t d = 64 * (blockIdx.y * (4 / SHARES) + wave / SHARES) + l, in = min(d, a.hd - 1);
   const uint32_t planes = wused * p.splits;
   const int64_t* src = p.planes + uint64_t(id) * a.hd + in;
@@ -906,8 +934,8 @@ __global__ __launch_bounds__(256) void k_tree_join(Launch p) {
   }
   if (d >= a.hd) return;
   y += uint64_t(end.extra * to_global(v)[d]);
-  if (end.n_big > 0) y += uint64_t(int64_t(to_global(row_ptr(s, s.v, a.v, a.kv_ld, end.big0, off))[d])) << 16;
-  if (end.n_big > 1) y += uint64_t(int64_t(to_global(row_ptr(s, s.v, a.v, a.kv_ld, end.big1, off))[d])) << 16;
+  if (end.n_big > 0) y += uint64_t(int64_t(to_global(values.at(end.big0))[d])) << 16;
+  if (end.n_big > 1) y += uint64_t(int64_t(to_global(values.at(end.big1))[d])) << 16;
   out[d] = end.first == kNone ? 0 : requant(int64_t(y));
 }
 
