@@ -178,13 +178,13 @@ __device__ __forceinline__ int64_t total(const v4i (&acc)[8], int r) {
 // requant(sum times by) of one component where the digits j have 0 .. 2 only, as
 // the whole double that it is: sums below 2^52 times scales are one rounded
 // multiply-add (the products of the integer form stay below 2^62, so that nothing
-// has wrapped there either). 8 instructions against 40.
+// has wrapped there either). About 12 instructions against 40.
 template <int P>
 __device__ __forceinline__ double scaled(const v4i (&acc)[8], int r, int32_t by, bool& far) {
-  // (at most 256 columns of 128 x 128 per pair, four pairs: words of two sums are below 2^32 / 2)
-  double y = double(acc[0][r] + (acc[1][r] << 8));
-  y = __builtin_fma(double(P > 1 ? acc[2][r] + (acc[3][r] << 8) : acc[2][r]), 65536.0, y);
-  if (P > 2) y = __builtin_fma(double(acc[4][r] + (acc[5][r] << 8)), 4294967296.0, y);
+  // (from the top: a partial sum past 2^53 leaves the whole one past 2^52)
+  double y = 0;
+#pragma unroll
+  for (int s = P + 1; s >= 0; --s) y = __builtin_fma(y, 256.0, double(acc[s][r]));
   const double b = double(by);
   far = far || !(__builtin_fabs(y) < 4503599627370496.0) || !(__builtin_fabs(y * b) < 4611686018427387904.0);
   return mul_rint(y, b * 0x1p-16);
@@ -194,7 +194,10 @@ __device__ __forceinline__ double scaled(const v4i (&acc)[8], int r, int32_t by,
 // columns each wave takes its 64 columns of the rows apart into LDS (the
 // weights' tile-steps: half h of step s, lane 16 g + i, holds columns 128 s +
 // 32 g + 16 h .. of row i); then wave w multiplies its rank tile with all of
-// them or its share. The next step's activations are on their way meanwhile.
+// them or its share. The next step's activations are on their way meanwhile. One
+// row of 2560 columns 4.2 us (latency), 1024 rows of 10240 columns and rank 64 in 16
+// bits 22.5 us, where the rows' 42 MB take 8.5 at a copy's rate: bound by the digits'
+// conversion and the LDS reads, four products per operand.
 template <int P>
 __device__ __forceinline__ void down_steps(const Plan& p, const DevAdapter& ad, const Tile& t, int8_t* lds,
                                            uint32_t* wide, uint32_t rank_tile, uint32_t part, uint32_t parts, bool on,

@@ -31,7 +31,9 @@ struct OpMaxU64 {
 // logits and mask bits are loaded before the rules are looked at. A token that
 // a rule names has its bit in `named` (history: `seen`) and its sum in `sum`:
 // minus its penalties, plus its biases; only those entries are ever written or
-// read. Bound by the logits' bytes.
+// read. Bound by the logits' bytes: 208 rows of 262144 tokens with histories,
+// biases and masks, adjusted logits written, 117 us, where copying them takes 81;
+// one row 6 us, a latency or two above an empty launch.
 template <bool VEC>
 __global__ __launch_bounds__(kThreads) void k_select(SelectArgs a, uint64_t* keys, uint32_t parts) {
   __shared__ unsigned long long sum[kSpan];

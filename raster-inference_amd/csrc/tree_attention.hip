@@ -248,9 +248,11 @@ __device__ __forceinline__ void score_tile(const v4i (&k)[NSUB][3], const v4i* q
 // the keys of one chunk, 16 per wave and step, which each wave loads and takes
 // apart in registers: no wave waits for another between its tiles. AHEAD: up to
 // 128 rows, half the waves, each step's keys loaded during the step before. At
-// 4096 rows of 8256 keys of 256 dims (16 sets of 256 rows) that takes 104 us
-// against 122 (the device copies its 330 MB, of which the scores are 135, in 67);
-// fewer than 65 rows leave the loads to twice the waves.
+// 4096 rows of 8256 keys of 256 dims (16 sets of 256 rows) that takes 102 us
+// against 122 (the device copies its 330 MB, of which the scores are 135, in 67).
+// Up to 64 rows both are as fast (28 rows of 2000 keys 8.6 and 8.7 us, 64 rows 14.2
+// and 13.3, 4 rows of 60 K keys for each of two heads 28 and 27, whose
+// 123 MB are 25 at a copy's rate).
 template <int NSUB, int MODE, bool AHEAD>
 __global__ __launch_bounds__(kThreads, NSUB <= 4 && !AHEAD ? 4 : 2) void k_tree_scores(Launch p) {
   extern __shared__ __attribute__((aligned(16))) int8_t lds[];  // [query tile][substep][digit][lane]
@@ -446,7 +448,7 @@ __device__ inline uint32_t seq_of(const Launch& p, uint32_t id) {
   return __builtin_amdgcn_readfirstlane(b);
 }
 
-// Terms of long rows: one wave per (row, chunk).
+// Terms of long rows: one wave per (row, chunk). 8 rows of 60 K keys: 5.8 us.
 __global__ __launch_bounds__(256) void k_tree_terms(Launch p) {
   const uint32_t l = threadIdx.x & 63, id = blockIdx.x * 4 + (threadIdx.x >> 6), chunk = blockIdx.y;
   if (id >= p.rows) return;
@@ -475,7 +477,7 @@ __global__ __launch_bounds__(256) void k_tree_terms(Launch p) {
       if (!plain) in = in && sees(v, s.rows, k);
       double e = 0;
       if (__any(in)) {
-        e = softmax_term_or_zero(gap, in);
+        e = softmax_term(gap, in);
         if (in && gap == 0) first = min(first, k);
         sum += e;
       }
@@ -571,9 +573,10 @@ __device__ inline int64_t residual(int64_t total, int64_t sum) {
 }
 // Whole rows: W waves turn a row's scores into weights through LDS, four
 // consecutive keys per lane; the weights' digits replace the scores in place (from
-// the row's start on). With rows enough to fill the device this reads
-// the scores once and writes half their bytes, where terms and weights by chunks
-// read and write 2.5 times as much.
+// the row's start on). With rows enough to fill the device this reads the scores
+// once and writes half their bytes, where terms and weights by chunks read and write
+// 2.5 times as much. 4096 rows of 8256 keys: 76 us, bound by about 60 instructions
+// per score (its 200 MB are 41 us at a copy's rate).
 constexpr uint32_t kRowKeys = 16384;  // most keys of a row (64 KB of terms)
 template <int W>
 __global__ __launch_bounds__(256) void k_tree_rows(Launch p, uint32_t lds_row) {
@@ -615,7 +618,7 @@ __global__ __launch_bounds__(256) void k_tree_rows(Launch p, uint32_t lds_row) {
       const bool seen = gap < (1u << 20) && ((vis >> q) & 1u);
       double y = 0;
       if (__any(seen)) {
-        y = softmax_term_or_zero(gap, seen);
+        y = softmax_term(gap, seen);
         if (__any(gap == 0)) {
           asm volatile("");
           if (seen && gap == 0) first = min(first, k + q);
@@ -657,7 +660,7 @@ __global__ __launch_bounds__(256) void k_tree_rows(Launch p, uint32_t lds_row) {
   }
 }
 
-// Weights of long rows: one wave per (row, chunk).
+// Weights of long rows: one wave per (row, chunk). 8 rows of 60 K keys: 4.8 us.
 __global__ __launch_bounds__(256) void k_tree_weights(Launch p) {
   const uint32_t l = threadIdx.x & 63, id = blockIdx.x * 4 + (threadIdx.x >> 6), chunk = blockIdx.y;
   if (id >= p.rows) return;
@@ -685,8 +688,11 @@ __global__ __launch_bounds__(256) void k_tree_weights(Launch p) {
 // consecutive bytes per key) a step ahead. The weights' digits (128 bytes per row
 // and step) come through a ring of three LDS stages, copied two steps ahead: 1 KB
 // slots of eight rows, of whose 16-byte pieces piece q of row r lies at place q ^
-// (r >> 1 & 7), so that the 16 rows of an operand read hit different banks. (Every
-// wave loading the digits of all rows into registers took 122 us instead of ..)
+// (r >> 1 & 7), so that the 16 rows of an operand read hit different banks. At 4096
+// rows of 8256 keys of 256 dims this takes 93 us (122 with every wave loading the
+// digits of all rows into registers), the 202 MB alone 41 at a copy's rate: the 128
+// sums of a lane leave two waves per SIMD, whose conversions and products overlap in
+// part only. 8 rows of 60 K keys (123 MB): 30 us, 25 at a copy's rate.
 constexpr int kStages = 3;
 template <int RT>
 __global__ __launch_bounds__(kThreads, 2) void k_tree_wsum(Launch p) {
@@ -883,7 +889,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_tree_wsum(Launch p) {
 }
 
 // Join: a wave per (row, 64 dims), or four with a share of the planes each where
-// there are many.
+// there are many. 4096 rows of 256 dims of four planes: 11.5 us for 38 MB, a wave's
+// few reads one after the other.
 template <int SHARES>
 __global__ __launch_bounds__(256) void k_tree_join(Launch p) {
   const uint32_t l = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -1012,6 +1019,8 @@ uint64_t plan(const TreeArgs& a, const TreeSeq* seqs, const Group& g, Launch& p)
   units = uint64_t(p.n_seq) * g.nkv * p.row_blocks;
   p.chunk = chunk_of(keys, units, p.block_rows > 64 ? 256 : 512, 16 * kWaves);
   p.chunks = uint32_t((keys + p.chunk - 1) / p.chunk);
+  // (28 rows of 3000 keys 32 us whole and 34 by chunks, of 6000 39 and 39, of 15000
+  // 51 and 46; 160 rows of 15000 84 and 86)
   p.whole = keys <= kRowKeys && (p.rows >= 256 || keys <= 4096);
   p.groups = a.hd <= 32 ? 1 : a.hd <= 64 ? 2 : a.hd <= 128 ? 4 : 8;
   p.splits = kWaves / p.groups;

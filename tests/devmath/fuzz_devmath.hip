@@ -84,8 +84,11 @@ int main(int argc, char** argv) {
   for (int64_t d = 0; d < (1 << 20); ++d) {
     int64_t o;
     orc_attention_softmax_exp_term(int32_t(-d), 0, &o);
-    if (det::softmax_term(uint32_t(d)) != double(o)) { bad++; if (bad < 5) printf("  softmax_term d=%lld\n", (long long)d); }
+    if (det::softmax_term(uint32_t(d), true) != double(o)) { bad++; if (bad < 5) printf("  softmax_term d=%lld\n", (long long)d); }
   }
+  // and none of an unwanted gap, whatever it is
+  for (int64_t k = 0; k < 1000000; ++k)
+    if (det::softmax_term(uint32_t(k < 4096 ? k << 20 : rng()), false) != 0) bad++;
   report("softmax_term_all_gaps", 1 << 20, bad);
   // sin_cos_rint: every quarter-turn border, random angles of all sizes
   bad = 0;

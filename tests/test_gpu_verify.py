@@ -45,11 +45,11 @@ def edges(rng, *shape):
 # ---------------------------------------------------------------------------
 def head_case(ctx, rng, hd, heads, rotary, layout, rows, positions, norm=True, gain=True, in_place=False, pad=0,
               shift=0, scaling=0, factor=ONE, low=0, high=0, original=0, amplitude=65536, base=10000 * ONE, eps=4295,
-              make=acts):
+              make=acts, gain_std=0.2):
     width = sum(heads) * hd
     stride = width + pad
     x = make(rng, rows, stride)
-    gains = [65536 + acts(rng, hd, std=0.2) if gain and i < 2 else None for i in range(len(heads))]
+    gains = [65536 + acts(rng, hd, std=gain_std) if gain and i < 2 else None for i in range(len(heads))]
     buf = ctx.to_device(np.concatenate([np.zeros(shift, np.int32), x.reshape(-1)]))
     out = buf if in_place else ctx.to_device(np.full(shift + rows * stride, 7, np.int32))
     table = rd.RopeTable(ctx, rotary, max(rotary, 2), base, layout=layout, scaling=scaling, factor=factor,
@@ -98,6 +98,29 @@ def test_head_norm_rope_shapes(ctx, layout, hd, heads, rotary):
 def test_head_norm_rope_options(ctx, layout, kw):
     rng = np.random.default_rng(17 + layout)
     head_case(ctx, rng, 64, (3, 2, 1), 48, layout, 4, [0, 5, 1_000_003, 2**32 - 1], **kw)
+
+
+# rows where a product saturates, or could: large values, results past 2^30 from large gains, scales past 2^21 from
+# tiny values, cosines above 2, all of them beside rows where none does
+def mixed(rng, rows, width):
+    x = acts(rng, rows, width, std=300.0 if rng.integers(2) else 1.0)
+    x[::2, : width // 2] = edges(rng, (rows + 1) // 2, width // 2)
+    return x
+
+
+def tiny(rng, rows, width):
+    return rng.integers(-2, 3, size=(rows, width)).astype(np.int32)
+
+
+@pytest.mark.parametrize("layout", [0, 1])
+@pytest.mark.parametrize("hd,heads,rotary", [(256, (6, 2, 2), 256), (256, (13, 1), 96), (96, (5, 1, 1), 96), (48, (9, 2), 24),
+                                             (30, (3, 2), 30), (512, (2, 1), 512), (768, (2, 1), 256)])
+@pytest.mark.parametrize("kw", [{"make": edges}, {"make": mixed}, {"make": tiny, "eps": 0}, {"gain_std": 9000.0},
+                                {"gain_std": 9000.0, "in_place": True}, {"amplitude": 200000}, {"amplitude": 131071},
+                                {"amplitude": 131072, "norm": False}, {"make": mixed, "norm": False, "in_place": True}])
+def test_head_norm_rope_saturates(ctx, layout, hd, heads, rotary, kw):
+    rng = np.random.default_rng(hd + rotary + layout)
+    head_case(ctx, rng, hd, heads, rotary, layout, 3, [3, 999, 123456], **kw)
 
 
 def test_head_norm_rope_equals_the_separate_primitives(ctx):
@@ -265,6 +288,63 @@ def test_tree_attention_long_cache(ctx, n):
     tree_case(ctx, rng, [n, 90], [2, 1], 2, 1, 64, starts=[0, n - 300, 5], q_std=0.05)
 
 
+@pytest.mark.parametrize("q,k,v", [(acts, acts, acts), (acts, edges, acts), (edges, acts, acts), (acts, acts, edges)])
+@pytest.mark.parametrize("hd,pad", [(64, 0), (100, 0), (192, 0), (256, 0), (256, 3), (320, 0)])
+def test_tree_attention_many_rows(ctx, q, k, v, hd, pad):
+    # more than 64 query rows of a head: blocks of 128 rows, whose keys are loaded a step ahead
+    tree_case(ctx, np.random.default_rng(hd + pad), [150, 20], [33, 9], 4, 1, hd, make_q=q, make_k=k, make_v=v, ring=(0,),
+              pad=pad, starts=np.arange(42) * 3)
+
+
+@pytest.mark.parametrize("n,drafts", [(4030, 1), (4097, 1), (5000, 64), (16330, 64), (16400, 64)])
+def test_tree_attention_whole_rows_and_chunks(ctx, n, drafts):
+    # rows turned into weights whole: up to 4096 keys, or 256 rows of up to 16384. The last, first and middle rows
+    # against the plain form, all of them against calls of eight rows
+    rng = np.random.default_rng(n)
+    heads, hd = 4, 16
+    k, v = acts(rng, n, hd), acts(rng, n, hd)
+    q, dk, dv = acts(rng, drafts, heads * hd, std=0.4), acts(rng, drafts, hd), acts(rng, drafts, hd)
+    masks = tree_masks(rng, [drafts])
+    starts = rng.integers(0, n, size=drafts).astype(np.uint32)
+    starts[::2] = 0
+    kb, vb, qb, dkb, dvb = (ctx.to_device(t) for t in (k, v, q, dk, dv))
+    mb, sb, out = ctx.to_device(masks), ctx.to_device(starts), ctx.empty((drafts, heads * hd))
+    view = rd.attn_caches([rd.AttnCache(kb, vb, hd, n)])
+    ctx.attention_tree(view, rd.u32_array([drafts]), qb, heads * hd, dkb, dvb, hd, mb, sb, heads, 1, hd, out, heads * hd)
+    got = out.numpy()
+    for i in {0, drafts // 2, drafts - 1}:
+        seen = [j for j in range(drafts) if int(masks[i]) >> j & 1]
+        keys, values = (np.concatenate([c[starts[i]:], d[seen]]) for c, d in ((k, dk), (v, dv)))
+        for h in (0, heads - 1):
+            c = slice(h * hd, (h + 1) * hd)
+            assert np.array_equal(got[i, c], ref.attention_row(q[i, c], keys, values)), (i, h)
+    # (two heads of a call at a time: half the rows)
+    half = ctx.empty((drafts, 2 * hd))
+    for h in (0, 2):
+        qh = ctx.to_device(np.ascontiguousarray(q[:, h * hd:(h + 2) * hd]))
+        ctx.attention_tree(view, rd.u32_array([drafts]), qh, 2 * hd, dkb, dvb, hd, mb, sb, 2, 1, hd, half, 2 * hd)
+        assert np.array_equal(got[:, h * hd:(h + 2) * hd], half.numpy())
+
+
+def test_tree_attention_scores_past_a_launch(ctx):
+    # 512 rows of 70030 keys for each of two kv heads are more score rows than a launch takes: a kv head at a time
+    rng = np.random.default_rng(21)
+    n, drafts, heads, kv_heads, hd = 69970, 64, 16, 2, 8
+    k, v = acts(rng, n, kv_heads * hd), acts(rng, n, kv_heads * hd)
+    q, dk, dv = acts(rng, drafts, heads * hd, std=0.5), acts(rng, drafts, kv_heads * hd), acts(rng, drafts, kv_heads * hd)
+    masks = tree_masks(rng, [drafts])
+    out = ctx.empty((drafts, heads * hd))
+    ctx.attention_tree(rd.attn_caches([rd.AttnCache(ctx.to_device(k), ctx.to_device(v), kv_heads * hd, n)]),
+                       rd.u32_array([drafts]), ctx.to_device(q), heads * hd, ctx.to_device(dk), ctx.to_device(dv),
+                       kv_heads * hd, ctx.to_device(masks), None, heads, kv_heads, hd, out, heads * hd)
+    got = out.numpy()
+    for i, h in [(0, 0), (63, 7), (30, 8), (63, 15)]:
+        seen = [j for j in range(drafts) if int(masks[i]) >> j & 1]
+        c, d = slice(h * hd, (h + 1) * hd), slice(h // 8 * hd, (h // 8 + 1) * hd)
+        keys, values = np.concatenate([k[:, d], dk[seen][:, d]]), np.concatenate([v[:, d], dv[seen][:, d]])
+        assert np.array_equal(got[i, c], ref.attention_row(q[i, c], keys, values)), (i, h)
+
+
 def test_tree_attention_offsets_past_32_bits(ctx):
     # rows 4194304 values apart: the last of 1100 lies past 2^32 values (17 GB)
     rng = np.random.default_rng(9)
@@ -424,6 +504,41 @@ def test_adapter_extremes(ctx, kinds):
                  scales=[I32_MAX, I32_MIN])
 
 
+@pytest.mark.parametrize("rank", [16, 128, 256])
+@pytest.mark.parametrize("value", [-32896, -128, 32639, -(2**23) - 2**15 - 128, 8355711])
+def test_adapter_digit_sums_at_their_ends(ctx, rank, value):
+    # h and B of one value whose digits are all the lowest or the highest
+    ones = np.full((rank, 1), 65536, dtype=np.int32)
+    up = np.full((20, rank), value if abs(value) < 2**16 else value // 512, dtype=np.int32)
+    x = np.array([[value], [-value]], dtype=np.int32)
+    w = np.zeros((20, 1), dtype=np.int32)
+    group = rd.Adapters(ctx, 20, 1, [rd.Adapter(ones, up, 65536)])
+    out = ctx.empty((2, 20))
+    ctx.det_linear_adapters(ctx.upload_matrix(w), group, 2, ctx.to_device(x), ctx.to_device(np.zeros(2, np.uint32)), out)
+    assert np.array_equal(out.numpy(), ref.linear_adapters(w, [(ones, up, 65536)], x, [0, 0]))
+
+
+@pytest.mark.parametrize("rows", [600, 5000, 20011])
+def test_adapter_outputs_per_workgroup(ctx, rows):
+    # one to four of B's tiles per wave, and rows of every adapter
+    rng = np.random.default_rng(rows)
+    adapter_case(ctx, rng, rows, 24, [3, 16, 20] * 6, 66, np.arange(66) % 19)
+
+
+def test_adapter_rows_in_ranges(ctx):
+    # more rows than a range of the call, of more adapters than threads that sort them
+    rng = np.random.default_rng(7)
+    m, rows, cols, n = 8200, 3, 5, 1100
+    w = weights(rng, rows, cols, "i16")
+    ads = [(weights(rng, 2, cols, "i16"), weights(rng, rows, 2, "i16")) for _ in range(n)]
+    index = rng.integers(0, n + 40, size=m).astype(np.uint32)
+    x = acts(rng, m, cols)
+    group = rd.Adapters(ctx, rows, cols, [rd.Adapter(a[0], b[0], 65536) for a, b in ads])
+    out = ctx.empty((m, rows))
+    ctx.det_linear_adapters(ctx.upload_matrix(w[0]), group, m, ctx.to_device(x), ctx.to_device(index), out)
+    assert np.array_equal(out.numpy(), ref.linear_adapters(w[2], [(a[2], b[2], 65536) for a, b in ads], x, index))
+
+
 def test_adapter_long_rows(ctx):
     rng = np.random.default_rng(3)
     adapter_case(ctx, rng, 20, 33000, [5], 3, [0, 0, 1])
@@ -547,6 +662,12 @@ def test_select_without_rules_is_argmax_first(ctx):
         ctx.select_tokens(xb, n, vocab, vocab, None, None, 0, tb)
         assert tb.numpy().tolist() == x.argmax(1).tolist()
         assert int(tb.numpy()[0]) == ctx.argmax_first(xb, vocab)
+
+
+@pytest.mark.parametrize("history,biases", [(2048, 0), (2049, 400), (7000, 700), (0, 900)])
+def test_select_long_rules(ctx, history, biases):
+    # histories and biases of more entries than a workgroup holds at a time
+    select_case(ctx, np.random.default_rng(history + biases), 2, 9000, history=history, biases=biases)
 
 
 def test_select_allowed_minimum_is_chosen_over_nothing(ctx):
