@@ -375,8 +375,9 @@ void launch(const HeadRopeArgs& a, hipStream_t s) {
 
 }  // namespace
 
-void launch_head_rope(const HeadRopeArgs& a, hipStream_t s) {
-  if (a.rows == 0 || a.total == 0) return;
+// (tokens in ranges: a grid has less than 2^32 threads)
+constexpr uint64_t kRange = uint64_t(1) << 22;
+static void launch_range(const HeadRopeArgs& a, hipStream_t s) {
   bool wide = a.hd % 4 == 0;
   for (uint32_t i = 0; i < a.n_sets; ++i) {
     const HeadSet& h = a.set[i];
@@ -392,6 +393,19 @@ void launch_head_rope(const HeadRopeArgs& a, hipStream_t s) {
     if (a.hd <= 64) launch<1, 1, 3>(a, s);
     else if (a.hd <= 256) launch<1, 4, 2>(a, s);
     else launch<1, 16, 1>(a, s);
+  }
+}
+void launch_head_rope(const HeadRopeArgs& a, hipStream_t s) {
+  if (a.total == 0) return;
+  HeadRopeArgs r = a;
+  for (uint64_t t = 0; t < a.rows; t += kRange) {
+    r.rows = std::min(a.rows - t, kRange);
+    if (a.positions) r.positions = a.positions + t;
+    for (uint32_t i = 0; i < a.n_sets; ++i) {
+      r.set[i].x = a.set[i].x + t * a.set[i].ld;
+      r.set[i].out = a.set[i].out + t * a.set[i].out_ld;
+    }
+    launch_range(r, s);
   }
 }
 

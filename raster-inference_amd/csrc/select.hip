@@ -57,8 +57,8 @@ __global__ __launch_bounds__(kThreads) void k_select(SelectArgs a, uint64_t* key
     }
   }
   if (biased) {
-    b0 = a.bias_begin[r];
     b1 = min(a.bias_begin[r + 1], n_bias);
+    b0 = min(a.bias_begin[r], b1);
   }
   // the batch of the row's history from entry `from` on (its spans one after the
   // other): offsets into this part, kSpan for other parts' tokens

@@ -136,6 +136,18 @@ def test_head_norm_rope_equals_the_separate_primitives(ctx):
     assert np.array_equal(a.numpy(), b.numpy())
 
 
+def test_head_norm_rope_of_more_rows_than_a_launch(ctx):
+    rng = np.random.default_rng(8)
+    rows, hd, some = (1 << 22) + 700, 4, 1009  # (rows and positions repeat)
+    x, positions = acts(rng, some, hd), np.arange(some, dtype=np.uint32) * 77
+    buf = ctx.to_device(np.resize(x, (rows, hd)))
+    table = rd.RopeTable(ctx, hd, hd, 10000 * ONE)
+    ctx.head_norm_rope(table, ctx.to_device(np.resize(positions, rows)), rows, hd, 4295, [rd.HeadRows(buf, hd, 1)])
+    freq = ref.frequencies(10000 * ONE, hd, hd // 2)
+    one = np.stack([ref.head_row(t, None, 4295, True, freq, int(p), 0, 65536, True) for t, p in zip(x, positions)])
+    assert np.array_equal(buf.numpy().reshape(rows, hd), np.resize(one, (rows, hd)))
+
+
 def test_head_norm_rope_without_rotation_or_rows(ctx):
     rng = np.random.default_rng(6)
     x = acts(rng, 5, 3 * 20)
@@ -697,6 +709,17 @@ def test_select_cuts_spans_and_biases_at_their_arrays(ctx):
     exp = np.zeros(64, dtype=np.int32)
     exp[2], exp[63] = -65536, 9
     assert np.array_equal(out.numpy()[0], exp) and tb.numpy()[0] == 63
+
+
+@pytest.mark.parametrize("begin", [2**32 - 1, 2**32 - 3, 2**32 - 515, 9, 2])
+def test_select_biases_that_begin_past_their_end(ctx, begin):
+    x = np.zeros((1, 40), dtype=np.int32)
+    rules = rd.LogitRules(bias_begin=ctx.to_device(np.array([begin, 2], dtype=np.uint32)),
+                          bias_ids=ctx.to_device(np.array([3, 7], dtype=np.uint32)),
+                          bias_values=ctx.to_device(np.array([5, 6], dtype=np.int32)), n_bias=2)
+    out = ctx.empty((1, 40))
+    ctx.select_tokens(ctx.to_device(x), 1, 40, 40, rules, out, 40, None)
+    assert not out.numpy().any()
 
 
 def test_select_refusals(ctx):
