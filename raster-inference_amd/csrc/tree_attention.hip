@@ -976,12 +976,31 @@ void for_groups(const TreeArgs& a, const TreeSeq* seqs, uint32_t n, F&& f) {
   }
 }
 
-// Keys per chunk: equal shares of the longest sequence, so that `units` blocks
-// per chunk make `want` blocks, what the device runs at once (in whole granules;
-// at most 16384 keys, which bounds the int32 sums and a wave's key tiles).
-uint32_t chunk_of(uint64_t keys, uint64_t units, uint64_t want, uint32_t granule) {
-  const uint64_t n = std::max<uint64_t>(want / units, 1);
-  return uint32_t(std::min<uint64_t>(up((keys + n - 1) / n, granule), 16384 / granule * granule));
+// Keys per chunk, in whole granules (at most 16384 keys, which bounds the int32
+// sums and a wave's key tiles): the share of the longest sequence, among some, that
+// ends first when the device runs `want` blocks at a time, each for its chunk and
+// `extra` keys' time besides. Ragged sequences leave a share of the longest one's
+// chunks empty.
+uint32_t chunk_of(const Launch& p, uint64_t keys, uint32_t block_rows, uint32_t dim_blocks, uint64_t want,
+                  uint32_t granule, uint32_t extra) {
+  uint64_t units = 0;
+  for (uint32_t b = 0; b < p.n_seq; ++b) units += (p.s[b].drafts * p.a.groups + block_rows - 1) / block_rows;
+  units *= uint64_t(p.nkv) * dim_blocks;
+  const uint64_t even = std::max<uint64_t>(want / units, 1);
+  uint64_t best = 0, least = UINT64_MAX, last = 0;
+  for (uint64_t n = even; n <= 4 * even; n += (even + 3) / 4) {
+    const uint64_t c = std::min<uint64_t>(up((keys + n - 1) / n, granule), 16384 / granule * granule);
+    if (c == last) continue;
+    last = c;
+    uint64_t blocks = 0;
+    for (uint32_t b = 0; b < p.n_seq; ++b)
+      blocks += ((p.s[b].drafts * p.a.groups + block_rows - 1) / block_rows) *
+                ((uint64_t(p.s[b].rows) + p.s[b].drafts + c - 1) / c);
+    blocks *= uint64_t(p.nkv) * dim_blocks;
+    const uint64_t cost = (blocks + want - 1) / want * (std::min(c, keys) + extra);
+    if (cost < least) least = cost, best = c;
+  }
+  return uint32_t(best);
 }
 
 // The launch of a group without its scratch pointers; returns the scratch's bytes.
@@ -991,7 +1010,7 @@ uint64_t plan(const TreeArgs& a, const TreeSeq* seqs, const Group& g, Launch& p)
   p.kv0 = g.kv0;
   p.nkv = g.nkv;
   p.n_seq = g.b1 - g.b0;
-  uint64_t scores = 0, keys = 0, units = 0;
+  uint64_t scores = 0, keys = 0;
   uint32_t most = 0;
   auto aligned = [](const void* q, uint64_t to) { return reinterpret_cast<uintptr_t>(q) % to == 0; };
   bool w4 = a.hd % 4 == 0 && a.q_ld % 4 == 0 && a.kv_ld % 4 == 0 && aligned(a.q, 16) && aligned(a.k, 16);
@@ -1016,8 +1035,7 @@ uint64_t plan(const TreeArgs& a, const TreeSeq* seqs, const Group& g, Launch& p)
   // their sums' registers would leave the device half empty
   p.block_rows = std::min<uint32_t>(uint32_t(up(most, 16)), a.hd <= 256 ? (most > 64 && w4 ? 128 : 64) : 32);
   p.row_blocks = (most + p.block_rows - 1) / p.block_rows;
-  units = uint64_t(p.n_seq) * g.nkv * p.row_blocks;
-  p.chunk = chunk_of(keys, units, p.block_rows > 64 ? 256 : 512, 16 * kWaves);
+  p.chunk = chunk_of(p, keys, p.block_rows, 1, p.block_rows > 64 ? 256 : 512, 16 * kWaves, 256);
   p.chunks = uint32_t((keys + p.chunk - 1) / p.chunk);
   // (28 rows of 3000 keys 32 us whole and 34 by chunks, of 6000 39 and 39, of 15000
   // 51 and 46; 160 rows of 15000 84 and 86)
@@ -1026,8 +1044,7 @@ uint64_t plan(const TreeArgs& a, const TreeSeq* seqs, const Group& g, Launch& p)
   p.splits = kWaves / p.groups;
   p.sum_rows = std::min<uint32_t>(uint32_t(up(most, 16)), a.hd <= 64 ? 32 : 64);
   p.sum_blocks = (most + p.sum_rows - 1) / p.sum_rows;
-  const uint64_t sums = uint64_t(p.n_seq) * g.nkv * p.sum_blocks * ((a.hd + kSumDims - 1) / kSumDims);
-  p.wchunk = chunk_of(keys, sums, 256, 64);
+  p.wchunk = chunk_of(p, keys, p.sum_rows, (a.hd + kSumDims - 1) / kSumDims, 256, 64, 128);
   p.splits = std::min(p.splits, p.wchunk / 64);
   p.wchunks = uint32_t((keys + p.wchunk - 1) / p.wchunk);
   uint64_t at = 0;
