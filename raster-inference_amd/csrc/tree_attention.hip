@@ -86,6 +86,7 @@ struct Launch {
   uint32_t sum_blocks, sum_rows;    // of the weighted sums
   int whole;                 // rows are turned into weights whole
   int wide_k, wide_v;  // 16-byte aligned q and k rows, 8-byte aligned v rows
+  int deep_v;          // 16-byte aligned v rows, more than 128 dims
   Seq s[kSeqs];
 };
 static_assert(sizeof(Launch) <= 4096, "kernel arguments");
@@ -694,7 +695,7 @@ __global__ __launch_bounds__(256) void k_tree_weights(Launch p) {
 // sums of a lane leave two waves per SIMD, whose conversions and products overlap in
 // part only. 8 rows of 60 K keys (123 MB): 30 us, 25 at a copy's rate.
 constexpr int kStages = 3;
-template <int RT>
+template <int RT, bool DEEP>
 __global__ __launch_bounds__(kThreads, 2) void k_tree_wsum(Launch p) {
   extern __shared__ __attribute__((aligned(16))) int8_t ring[];  // [stage][split][row][128]
   const Item it = item_of(p, p.wchunks, p.sum_blocks);
@@ -760,6 +761,28 @@ __global__ __launch_bounds__(kThreads, 2) void k_tree_wsum(Launch p) {
           (void __attribute__((address_space(3)))*)(ring + ((st % kStages) * slots + c) * kOp), 16, 0, 0);
     }
   };
+  // DEEP: the wave's values of step `st`, into one of two LDS stages: 128 bytes per
+  // key (16 per lane, eight keys per copy), keys 16 g + e with odd g at place 16 g +
+  // (e ^ 1), so that two groups of lanes read from different banks
+  constexpr uint32_t kValueBytes = 64 * 128;
+  int8_t* vring = ring + kStages * slots * kOp;
+  const uint32_t piece = min(dim0 + 4 * (l % 8), hd >= 4 ? hd - 4 : 0);
+  auto copy_v = [&](uint32_t st) {
+    const uint32_t k = k0 + 64 * st;
+    int8_t* dst = vring + ((st & 1) * kWaves + wave) * kValueBytes;
+    uint64_t at = s.first + k;
+    if (s.wrap && at >= s.wrap) at -= s.wrap;
+    const bool run = k + 64 <= s.rows && (!s.wrap || at + 64 <= s.wrap) && s.ld < (1u << 22);
+    const int32_t* base = s.v + at * s.ld + off;
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) {
+      const uint32_t key = (l / 8) ^ (e / 2 & 1);
+      const int32_t* src = run ? base + 8 * e * s.ld + (key * uint32_t(s.ld) + piece)
+                               : values.at(min(k + 8 * e + key, n - 1)) + piece;
+      __builtin_amdgcn_global_load_lds((const void __attribute__((address_space(1)))*)src,
+                                       (void __attribute__((address_space(3)))*)(dst + e * kOp), 16, 0, 0);
+    }
+  };
   auto digit_words = [&](const int32_t (&x)[16][2], int c, v4i (&d)[4], uint32_t& all) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -792,22 +815,48 @@ __global__ __launch_bounds__(kThreads, 2) void k_tree_wsum(Launch p) {
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
+  // (DEEP: one share, so that a wave is on in every step or in none; nine copies a step, or one)
+  if (DEEP && on) copy_v(0);
   copy_w(0);
+  if (DEEP && on && steps > 1) copy_v(1);
   if (steps > 1) copy_w(1);
-  if (on) load_v(k0, x);
+  if (!DEEP && on) load_v(k0, x);
 #pragma unroll 1
   for (uint32_t st = 0; st < steps; ++st) {
+    const uint32_t k = k0 + 64 * st;
     v4i d[2][4];
+    if (DEEP) {
+      // this step's copies; the next one's may be on their way
+      asm volatile("" ::: "memory");
+      if (st + 1 == steps) __builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (15 << 8));
+      else if (on) __builtin_amdgcn_s_waitcnt(9 | (7 << 4) | (15 << 8));
+      else __builtin_amdgcn_s_waitcnt(1 | (7 << 4) | (15 << 8));
+      if (wave < kWaves / 2) __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      const int8_t* src = vring + ((st & 1) * kWaves + wave) * kValueBytes + 8 * i;
+#pragma unroll
+      for (uint32_t e = 0; e < 16; ++e) {
+        const int2 t = *reinterpret_cast<const int2*>(src + ((16 * g + e) ^ (g & 1)) * 128);
+        x[e][0] = t.x, x[e][1] = t.y;
+      }
+    }
     digit_words(x, 0, d[0], all);
     digit_words(x, 1, d[1], all);
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int q = 0; q < 3; ++q) asm volatile("" : "+v"(d[c][q]));
-    step_barrier();
-    if (st + 2 < steps) copy_w(st + 2);
-    const uint32_t k = k0 + 64 * st;
-    if (on && k + 64 < k1) load_v(k + 64, x);
+    if (DEEP) {
+      asm volatile("" ::: "memory");
+      if (on && st + 2 < steps) copy_v(st + 2);
+      if (wave >= kWaves / 2) __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (st + 2 < steps) copy_w(st + 2);
+    } else {
+      step_barrier();
+      if (st + 2 < steps) copy_w(st + 2);
+      if (on && k + 64 < k1) load_v(k + 64, x);
+    }
     if (on && k < k1)
 #pragma unroll
       for (int T = 0; T < RT; ++T) {
@@ -1015,6 +1064,7 @@ uint64_t plan(const TreeArgs& a, const TreeSeq* seqs, const Group& g, Launch& p)
   auto aligned = [](const void* q, uint64_t to) { return reinterpret_cast<uintptr_t>(q) % to == 0; };
   bool w4 = a.hd % 4 == 0 && a.q_ld % 4 == 0 && a.kv_ld % 4 == 0 && aligned(a.q, 16) && aligned(a.k, 16);
   bool w2 = a.hd % 2 == 0 && a.kv_ld % 2 == 0 && aligned(a.v, 8);
+  bool v4 = a.hd % 4 == 0 && a.kv_ld % 4 == 0 && aligned(a.v, 16);
   for (uint32_t b = g.b0; b < g.b1; ++b) {
     const TreeSeq& t = seqs[b];
     Seq& s = p.s[b - g.b0];
@@ -1022,6 +1072,7 @@ uint64_t plan(const TreeArgs& a, const TreeSeq* seqs, const Group& g, Launch& p)
     if (t.rows) {
       w4 = w4 && t.ld % 4 == 0 && aligned(t.k, 16);
       w2 = w2 && t.ld % 2 == 0 && aligned(t.v, 8);
+      v4 = v4 && t.ld % 4 == 0 && aligned(t.v, 16);
     }
     const uint32_t R = t.drafts * a.groups;
     p.rows += R * g.nkv;
@@ -1031,6 +1082,7 @@ uint64_t plan(const TreeArgs& a, const TreeSeq* seqs, const Group& g, Launch& p)
   }
   p.wide_k = w4;
   p.wide_v = w2;
+  p.deep_v = v4 && a.hd > 128;
   // 64 query rows per block, 128 with loads a step ahead; 32 where their digits or
   // their sums' registers would leave the device half empty
   p.block_rows = std::min<uint32_t>(uint32_t(up(most, 16)), a.hd <= 256 ? (most > 64 && w4 ? 128 : 64) : 32);
@@ -1083,10 +1135,14 @@ void launch_scores(const Launch& p, uint32_t blocks, hipStream_t s) {
 }
 template <int RT>
 void launch_wsum(const Launch& p, uint32_t blocks, hipStream_t s) {
-  (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&k_tree_wsum<RT>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                            128 << 10);
-  hipLaunchKernelGGL(k_tree_wsum<RT>, dim3(blocks, (p.a.hd + kSumDims - 1) / kSumDims), dim3(kThreads),
-                     kStages * p.splits * RT * 2 * kOp, s, p);
+  const uint32_t lds = kStages * p.splits * RT * 2 * kOp;
+  auto go = [&](auto kernel, uint32_t bytes) {
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 156 << 10);
+    hipLaunchKernelGGL(kernel, dim3(blocks, (p.a.hd + kSumDims - 1) / kSumDims), dim3(kThreads), bytes, s, p);
+  };
+  if constexpr (RT == 4)
+    if (p.deep_v) return go(&k_tree_wsum<RT, true>, lds + 2 * kWaves * 8192);
+  go(&k_tree_wsum<RT, false>, lds);
 }
 void launch_rows(const Launch& p, hipStream_t s) {
   uint32_t ld = 0;
