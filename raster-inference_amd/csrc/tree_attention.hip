@@ -685,15 +685,19 @@ __global__ __launch_bounds__(256) void k_tree_weights(Launch p) {
 
 // Weighted sums: a block takes up to 16 RT query rows, one chunk of keys and
 // 256 head dims; each wave a group of 32 dims and a split of the keys, 64 of
-// them per step. Lane 16 g + i loads dims 2 i, 2 i + 1 of the keys 16 g + e (128
-// consecutive bytes per key) a step ahead. The weights' digits (128 bytes per row
-// and step) come through a ring of three LDS stages, copied two steps ahead: 1 KB
-// slots of eight rows, of whose 16-byte pieces piece q of row r lies at place q ^
-// (r >> 1 & 7), so that the 16 rows of an operand read hit different banks. At 4096
-// rows of 8256 keys of 256 dims this takes 93 us (122 with every wave loading the
-// digits of all rows into registers), the 202 MB alone 41 at a copy's rate: the 128
-// sums of a lane leave two waves per SIMD, whose conversions and products overlap in
-// part only. 8 rows of 60 K keys (123 MB): 30 us, 25 at a copy's rate.
+// them per step. Lane 16 g + i has dims 2 i, 2 i + 1 of the keys 16 g + e (128
+// consecutive bytes per key), loaded a step ahead. The weights' digits (128 bytes
+// per row and step) come through a ring of three LDS stages, copied two steps
+// ahead: 1 KB slots of eight rows, of whose 16-byte pieces piece q of row r lies at
+// place q ^ (r >> 1 & 7), so that the 16 rows of an operand read hit different banks.
+// DEEP: 64 rows of more than 128 dims, where the 128 sums of a lane leave two waves
+// per SIMD: the values come through LDS as well, two steps ahead, and the second half
+// of the waves pass each step's barrier after their conversions instead of before, so
+// that of a SIMD's two waves one converts while the other multiplies. At 4096 rows of
+// 8256 keys of 256 dims that takes 78 us, 89 with all waves in phase, 93 with values
+// loaded a step ahead and 122 with the digits loaded by every wave; the bytes alone (67
+// MB of digits, 135 of values) take 41. One row of each of 8 heads over 60 K keys (123
+// MB): 30 us, 25 at a copy's rate.
 constexpr int kStages = 3;
 template <int RT, bool DEEP>
 __global__ __launch_bounds__(kThreads, 2) void k_tree_wsum(Launch p) {
