@@ -357,6 +357,37 @@ def test_tree_attention_scores_past_a_launch(ctx):
         assert np.array_equal(got[i, c], ref.attention_row(q[i, c], keys, values)), (i, h)
 
 
+@pytest.mark.parametrize("cached,drafts,ring,hd,v", [
+    ([1500, 700], [20, 17], (0, 1), 256, acts), ([640, 64, 63], [14, 64, 9], (), 256, acts), ([900], [33], (0,), 132, acts),
+    ([333, 1], [12, 12], (0,), 512, acts), ([450, 200], [16, 9], (1,), 256, edges)])
+def test_tree_attention_long_values(ctx, cached, drafts, ring, hd, v):
+    # more than 32 query rows of more than 128 dims: the values come through LDS, over many steps, rings that wrap
+    # inside a step and drafted rows at the end of one
+    rng = np.random.default_rng(sum(cached) + hd)
+    tree_case(ctx, rng, cached, drafts, 4, 1, hd, ring=ring, make_v=v)
+
+
+def test_tree_attention_far_apart_rows(ctx):
+    # rows too far apart for 32-bit offsets of a step, of more than 32 query rows
+    rng = np.random.default_rng(13)
+    heads, hd, n, stride, d = 16, 160, 70, 1 << 22, 3
+    big = ctx.alloc((n - 1) * stride * 4 + 2 * hd * 4)
+    k, v = acts(rng, n, hd), acts(rng, n, hd)
+    for r in range(n):
+        for i, t in enumerate((k, v)):
+            row = np.ascontiguousarray(t[r])
+            ctx.check(ctx.lib.det_memcpy_h2d(ctx.handle, rd.C.c_void_p(big.ptr + (r * stride + i * hd) * 4),
+                                             rd._ptr(row), row.nbytes))
+    q, dk, dv = acts(rng, d, heads * hd, std=0.2), acts(rng, d, hd), acts(rng, d, hd)
+    masks = np.array([1, 3, 5], dtype=np.uint64)
+    out = ctx.empty((d, heads * hd))
+    ctx.attention_tree(rd.attn_caches([rd.AttnCache(big, At(big, hd), stride, n)]), rd.u32_array([d]), ctx.to_device(q),
+                       heads * hd, ctx.to_device(dk), ctx.to_device(dv), hd, ctx.to_device(masks), None, heads, 1, hd, out,
+                       heads * hd)
+    assert np.array_equal(out.numpy(), ref.attention_tree([(k, v)], [d], q, dk, dv, masks, None, heads, 1, hd))
+    big.free()
+
+
 def test_tree_attention_offsets_past_32_bits(ctx):
     # rows 4194304 values apart: the last of 1100 lies past 2^32 values (17 GB)
     rng = np.random.default_rng(9)
