@@ -260,7 +260,7 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 && !AHEAD ? 4 : 2) void k_tree_
   constexpr uint32_t kRows = AHEAD ? 128 : 64;
   __shared__ int32_t rmax[kRows];  // each row's largest score so far
   __shared__ Sight sight[kRows];
-  __shared__ uint32_t qwide, last_start;
+  __shared__ uint32_t qwide[kWaves], last_start;
   const Item it = item_of(p, p.chunks, p.row_blocks);
   if (!it.on) return;
   const Seq& s = p.s[it.seq];
@@ -271,6 +271,23 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 && !AHEAD ? 4 : 2) void k_tree_
   const uint32_t rows = min(R - r0, p.block_rows), tiles = (rows + 15) / 16;
   const uint32_t tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = l & 15, g = l >> 4;
   const uint32_t kvh = p.kv0 + it.kvh, hd = a.hd;
+  const uint64_t off = uint64_t(kvh) * hd;
+  const Rows keys(s, s.k, a.k, a.kv_ld, off);
+  int32_t x[NSUB][4][4];
+  auto load_k = [&](uint32_t key0) {
+    const int32_t* src = keys.at(key0 + i);
+    uint32_t hdl = hd;
+    if (MODE != kWhole) asm volatile("" : "+s"(hdl));  // (offsets kept over the loop would spill)
+#pragma unroll
+    for (int sub = 0; sub < NSUB; ++sub)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // (the rows' last substep only can pass their end, but for the eight of 257 to 512 dims)
+        if (MODE == kVec4 && sub + 1 < NSUB && NSUB < 8) load4<kWhole>(src, 64 * sub + 16 * j + 4 * g, hd, x[sub][j]);
+        else load4<MODE>(src, 64 * sub + 16 * j + 4 * g, hdl, x[sub][j]);
+        if (MODE == kScalar) __builtin_amdgcn_sched_barrier(0);  // (addresses of four values at a time)
+      }
+  };
   if (tid < 64) {
     uint32_t m = 0;
 #pragma unroll
@@ -281,9 +298,8 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 && !AHEAD ? 4 : 2) void k_tree_
       rmax[r] = INT32_MIN;
     }
     m = uint32_t(wave_max64(int64_t(m)));
-    if (tid == 0) qwide = 0, last_start = m;
+    if (tid == 0) last_start = m;
   }
-  __syncthreads();
   // this lane's row of query tile T, and its values [dim, dim + 4)
   auto q_row = [&](uint32_t T) {
     const uint32_t row = min(r0 + 16 * T + i, R - 1);
@@ -295,30 +311,30 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 && !AHEAD ? 4 : 2) void k_tree_
     for (int e = 0; e < 4; ++e)
       if (dim + e >= hd) x[e] = 0;
   };
+  uint32_t q_all = 0;
   for (uint32_t u = wave; u < tiles * NSUB; u += kWaves) {
     const uint32_t sub = u % NSUB;
     const int32_t* src = q_row(u / NSUB);
-    uint32_t d[3][4], all = 0;
+    uint32_t d[3][4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      int32_t x[4];
-      load_q(src, 64 * sub + 16 * j + 4 * g, x);
+      int32_t y[4];
+      load_q(src, 64 * sub + 16 * j + 4 * g, y);
       uint32_t w[4];
-      digits4(x, w, all);
+      digits4(y, w, q_all);
 #pragma unroll
       for (int q = 0; q < 3; ++q) d[q][j] = w[q];
     }
     v4i* dst = reinterpret_cast<v4i*>(lds) + uint64_t(u) * 3 * 64 + l;
 #pragma unroll
     for (int q = 0; q < 3; ++q) dst[q * 64] = v4i{int(d[q][0]), int(d[q][1]), int(d[q][2]), int(d[q][3])};
-    if (__any(all != 0) && l == 0) qwide = 1;
   }
-  __syncthreads();
-  const bool qw = qwide != 0;
+  const bool q_any = __any(q_all != 0);
+  if (l == 0) qwide[wave] = q_any;
+  lds_barrier();
+  const bool qw = __any(qwide[l % kWaves] != 0);
   const uint32_t id0 = s.id0 + it.kvh * R + r0;
   int32_t* sc = p.scores + s.score0 + uint64_t(it.kvh * R + r0) * s.score_ld;
-  const uint64_t off = uint64_t(kvh) * hd;
-  const Rows keys(s, s.k, a.k, a.kv_ld, off);
   const uint32_t seen_from = __builtin_amdgcn_readfirstlane(last_start);
   // scores of tile T and the keys from key0 on: stored, and the largest seen one kept
   auto finish = [&](uint32_t T, uint32_t key0, const int32_t (&out)[4]) {
@@ -337,21 +353,6 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 && !AHEAD ? 4 : 2) void k_tree_
     atomicMax(&rmax[16 * T + i], m);
   };
   uint64_t later0 = 0, later1 = 0;  // key tiles that are not narrow (at most 128 per wave and chunk; wave-uniform)
-  int32_t x[NSUB][4][4];
-  auto load_k = [&](uint32_t key0) {
-    const int32_t* src = keys.at(key0 + i);
-    uint32_t hdl = hd;
-    if (MODE != kWhole) asm volatile("" : "+s"(hdl));  // (offsets kept over the loop would spill)
-#pragma unroll
-    for (int sub = 0; sub < NSUB; ++sub)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        // (the rows' last substep only can pass their end, but for the eight of 257 to 512 dims)
-        if (MODE == kVec4 && sub + 1 < NSUB && NSUB < 8) load4<kWhole>(src, 64 * sub + 16 * j + 4 * g, hd, x[sub][j]);
-        else load4<MODE>(src, 64 * sub + 16 * j + 4 * g, hdl, x[sub][j]);
-        if (MODE == kScalar) __builtin_amdgcn_sched_barrier(0);  // (addresses of four values at a time)
-      }
-  };
   if (AHEAD && k0 + 16 * wave < k1) load_k(k0 + 16 * wave);
   for (uint32_t key0 = k0 + 16 * wave, t = 0; key0 < k1; key0 += 16 * kWaves, ++t) {
     v4i k3[NSUB][3];
@@ -576,7 +577,7 @@ __device__ inline int64_t residual(int64_t total, int64_t sum) {
 // consecutive keys per lane; the weights' digits replace the scores in place (from
 // the row's start on). With rows enough to fill the device this reads the scores
 // once and writes half their bytes, where terms and weights by chunks read and write
-// 2.5 times as much. 4096 rows of 8256 keys: 76 us, bound by about 60 instructions
+// 2.5 times as much. 4096 rows of 8256 keys: 73 us, bound by about 60 instructions
 // per score (its 200 MB are 41 us at a copy's rate).
 constexpr uint32_t kRowKeys = 16384;  // most keys of a row (64 KB of terms)
 template <int W>
@@ -592,18 +593,20 @@ __global__ __launch_bounds__(256) void k_tree_rows(Launch p, uint32_t lds_row) {
   const Seq& s = p.s[seq_of(p, id)];
   const uint32_t R = s.drafts * p.a.groups, local = id - s.id0, n = s.rows + s.drafts, n64 = (n + 63) & ~63u;
   const uint32_t used = (n + p.chunk - 1) / p.chunk;
+  int32_t* sc = p.scores + s.score0 + uint64_t(local) * s.score_ld;
+  // (each step's scores are loaded before the step that uses the ones before)
+  int4 t = 4 * lane < n64 ? *reinterpret_cast<const int4*>(sc + 4 * lane) : make_int4(0, 0, 0, 0);
   int32_t m = INT32_MIN;
   for (uint32_t c = l; c < used; c += 64) m = max(m, p.pmax[uint64_t(id) * p.chunks + c]);
   const Sight v = sight_of(p.a, s, local % R / p.a.groups);
   m = int32_t(wave_max64(m));
-  int32_t* sc = p.scores + s.score0 + uint64_t(local) * s.score_ld;
   uint32_t* terms = row_terms + in * lds_row;
   if (lane == 0) ends[in].n_big = 0;
   double sum = 0;  // (whole numbers below 2^53: exact in any order)
   uint32_t first = kNone;
   for (uint32_t k = 4 * lane; k < n64; k += 256 * W) {
-    const int4 t = *reinterpret_cast<const int4*>(sc + k);
     const int32_t x[4] = {t.x, t.y, t.z, t.w};
+    if (k + 256 * W < n64) t = *reinterpret_cast<const int4*>(sc + k + 256 * W);
     uint32_t e[4];
     // what of the four keys is seen
     uint32_t vis = k >= v.start && k + 4 <= s.rows ? 15u : 0u;
