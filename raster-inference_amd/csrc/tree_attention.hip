@@ -56,7 +56,6 @@ struct Seq {
   uint64_t row0;     // first drafted row
   uint64_t score0;   // first value of its score rows
   uint32_t rows, drafts;
-  uint32_t id0;      // row id of its first row
   uint32_t score_ld;
 };
 // What a row's output has besides its two-digit weights.
@@ -79,34 +78,44 @@ struct Launch {
   RowEnd* ends;        // [row id]
   uint32_t kv0, nkv;   // kv heads of the launch
   uint32_t n_seq, rows;  // row ids
-  uint32_t chunk, chunks;    // keys per chunk of the scores and terms
-  uint32_t wchunk, wchunks;  // of the weighted sums
+  uint32_t chunk, chunks, items;     // keys per chunk of the scores and terms
+  uint32_t wchunk, wchunks, witems;  // of the weighted sums
   uint32_t splits, groups;   // waves of a weighted-sum block: key splits x groups of 32 dims
   uint32_t row_blocks, block_rows;  // of the scores
   uint32_t sum_blocks, sum_rows;    // of the weighted sums
   int whole;                 // rows are turned into weights whole
   int wide_k, wide_v;  // 16-byte aligned q and k rows, 8-byte aligned v rows
   int deep_v;          // 16-byte aligned v rows, more than 128 dims
+  // per sequence: the row id of its first row, the first of its items (chunks x kv
+  // heads) in the scores and in the weighted sums
+  uint32_t id0[kSeqs], item0[kSeqs], witem0[kSeqs];
   Seq s[kSeqs];
 };
 static_assert(sizeof(Launch) <= 4096, "kernel arguments");
 
-// The work item of this workgroup: items (sequence, kv head, chunk) go round
+// The sequence that number `at` belongs to, of the sequences' first ones (a vector
+// load and a ballot: reading them one after the other takes a latency each).
+__device__ inline uint32_t find_seq(const uint32_t (&first)[kSeqs], uint32_t n_seq, uint32_t at) {
+  const uint32_t l = threadIdx.x & 63, v = first[min(l, kSeqs - 1)];
+  return uint32_t(__popcll(__ballot(l < n_seq && v <= at))) - 1;
+}
+// The work item of this workgroup: items (sequence, chunk, kv head) go round
 // the eight XCDs, an item's row blocks one after the other on one XCD, so that
 // they find its keys in that XCD's L2.
 struct Item {
   uint32_t seq, kvh, chunk, rb;
   bool on;
 };
-__device__ inline Item item_of(const Launch& p, uint32_t chunks, uint32_t row_blocks) {
+__device__ inline Item item_of(const Launch& p, const uint32_t (&item0)[kSeqs], uint32_t items, uint32_t row_blocks) {
   const uint32_t id = blockIdx.x, w = (id / 8 / row_blocks) * 8 + id % 8;
-  Item it;
+  Item it{};
+  it.on = w < items;
+  if (!it.on) return it;
   it.rb = id / 8 % row_blocks;
-  it.chunk = w % chunks;
-  const uint32_t u = w / chunks;
+  it.seq = p.n_seq > 1 ? find_seq(item0, p.n_seq, w) : 0;
+  const uint32_t u = w - (p.n_seq > 1 ? item0[it.seq] : 0);
   it.kvh = u % p.nkv;
-  it.seq = u / p.nkv;
-  it.on = it.seq < p.n_seq;
+  it.chunk = u / p.nkv;
   return it;
 }
 
@@ -261,7 +270,7 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 && !AHEAD ? 4 : 2) void k_tree_
   __shared__ int32_t rmax[kRows];  // each row's largest score so far
   __shared__ Sight sight[kRows];
   __shared__ uint32_t qwide[kWaves], last_start;
-  const Item it = item_of(p, p.chunks, p.row_blocks);
+  const Item it = item_of(p, p.item0, p.items, p.row_blocks);
   if (!it.on) return;
   const Seq& s = p.s[it.seq];
   const TreeArgs& a = p.a;
@@ -333,7 +342,7 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 && !AHEAD ? 4 : 2) void k_tree_
   if (l == 0) qwide[wave] = q_any;
   lds_barrier();
   const bool qw = __any(qwide[l % kWaves] != 0);
-  const uint32_t id0 = s.id0 + it.kvh * R + r0;
+  const uint32_t id0 = p.id0[it.seq] + it.kvh * R + r0;
   int32_t* sc = p.scores + s.score0 + uint64_t(it.kvh * R + r0) * s.score_ld;
   const uint32_t seen_from = __builtin_amdgcn_readfirstlane(last_start);
   // scores of tile T and the keys from key0 on: stored, and the largest seen one kept
@@ -443,19 +452,13 @@ __global__ __launch_bounds__(kThreads, NSUB <= 4 && !AHEAD ? 4 : 2) void k_tree_
 // An exp term (at most 2^32, and otherwise below 2^32 - 65000) from its 32 bits.
 __device__ inline int64_t unpack_term(uint32_t e) { return int64_t(uint64_t(e) + (e == 0xffffffffu)); }
 
-// The sequence and place of a row id (wave-uniform).
-__device__ inline uint32_t seq_of(const Launch& p, uint32_t id) {
-  uint32_t b = 0;
-  while (b + 1 < p.n_seq && p.s[b + 1].id0 <= id) ++b;
-  return __builtin_amdgcn_readfirstlane(b);
-}
-
 // Terms of long rows: one wave per (row, chunk). 8 rows of 60 K keys: 5.8 us.
 __global__ __launch_bounds__(256) void k_tree_terms(Launch p) {
   const uint32_t l = threadIdx.x & 63, id = blockIdx.x * 4 + (threadIdx.x >> 6), chunk = blockIdx.y;
   if (id >= p.rows) return;
-  const Seq& s = p.s[seq_of(p, id)];
-  const uint32_t R = s.drafts * p.a.groups, local = id - s.id0, n = s.rows + s.drafts;
+  const uint32_t seq = find_seq(p.id0, p.n_seq, id);
+  const Seq& s = p.s[seq];
+  const uint32_t R = s.drafts * p.a.groups, local = id - p.id0[seq], n = s.rows + s.drafts;
   const uint32_t k0 = chunk * p.chunk, k1 = min(k0 + p.chunk, n);
   if (k0 >= k1) return;
   const uint32_t used = (n + p.chunk - 1) / p.chunk;
@@ -590,8 +593,9 @@ __global__ __launch_bounds__(256) void k_tree_rows(Launch p, uint32_t lds_row) {
   const uint32_t l = threadIdx.x & 63, wave = threadIdx.x >> 6, in = wave / W, lane = threadIdx.x % (64 * W);
   const uint32_t id = __builtin_amdgcn_readfirstlane(min(blockIdx.x * (4 / W) + in, p.rows - 1));
   const bool on = blockIdx.x * (4 / W) + in < p.rows;
-  const Seq& s = p.s[seq_of(p, id)];
-  const uint32_t R = s.drafts * p.a.groups, local = id - s.id0, n = s.rows + s.drafts, n64 = (n + 63) & ~63u;
+  const uint32_t seq = find_seq(p.id0, p.n_seq, id);
+  const Seq& s = p.s[seq];
+  const uint32_t R = s.drafts * p.a.groups, local = id - p.id0[seq], n = s.rows + s.drafts, n64 = (n + 63) & ~63u;
   const uint32_t used = (n + p.chunk - 1) / p.chunk;
   int32_t* sc = p.scores + s.score0 + uint64_t(local) * s.score_ld;
   // (each step's scores are loaded before the step that uses the ones before)
@@ -668,8 +672,9 @@ __global__ __launch_bounds__(256) void k_tree_rows(Launch p, uint32_t lds_row) {
 __global__ __launch_bounds__(256) void k_tree_weights(Launch p) {
   const uint32_t l = threadIdx.x & 63, id = blockIdx.x * 4 + (threadIdx.x >> 6), chunk = blockIdx.y;
   if (id >= p.rows) return;
-  const Seq& s = p.s[seq_of(p, id)];
-  const uint32_t local = id - s.id0, n = s.rows + s.drafts, used = (n + p.chunk - 1) / p.chunk;
+  const uint32_t seq = find_seq(p.id0, p.n_seq, id);
+  const Seq& s = p.s[seq];
+  const uint32_t local = id - p.id0[seq], n = s.rows + s.drafts, used = (n + p.chunk - 1) / p.chunk;
   const uint32_t k0 = chunk * p.chunk, k2 = min((min(k0 + p.chunk, n) + 63) & ~63u, s.score_ld);
   if (k0 >= n) return;
   int64_t sum = 0;
@@ -705,7 +710,7 @@ constexpr int kStages = 3;
 template <int RT, bool DEEP>
 __global__ __launch_bounds__(kThreads, 2) void k_tree_wsum(Launch p) {
   extern __shared__ __attribute__((aligned(16))) int8_t ring[];  // [stage][split][row][128]
-  const Item it = item_of(p, p.wchunks, p.sum_blocks);
+  const Item it = item_of(p, p.witem0, p.witems, p.sum_blocks);
   if (!it.on) return;
   const Seq& s = p.s[it.seq];
   const TreeArgs& a = p.a;
@@ -719,7 +724,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_tree_wsum(Launch p) {
   const uint32_t steps = ((c1 - c0 + 63) / 64 + splits - 1) / splits;
   const uint32_t k0 = c0 + split * steps * 64, k1 = min(k0 + steps * 64, c1);
   const bool on = split < splits && dim0 < hd && k0 < k1;
-  const uint32_t rows = min(R - r0, p.sum_rows), id0 = s.id0 + it.kvh * R + r0;
+  const uint32_t rows = min(R - r0, p.sum_rows), id0 = p.id0[it.seq] + it.kvh * R + r0;
   const uint64_t off = uint64_t(kvh) * hd;
   const Rows values(s, s.v, a.v, a.kv_ld, off);
   const uint32_t dim = dim0 + 2 * i, dim_in = dim + 1 < hd ? dim : (hd > 1 ? hd - 2 : 0);  // (sums of dims past hd are dropped)
@@ -951,9 +956,10 @@ template <int SHARES>
 __global__ __launch_bounds__(256) void k_tree_join(Launch p) {
   const uint32_t l = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t id = blockIdx.x;
-  const Seq& s = p.s[seq_of(p, id)];
+  const uint32_t seq = find_seq(p.id0, p.n_seq, id);
+  const Seq& s = p.s[seq];
   const TreeArgs& a = p.a;
-  const uint32_t R = s.drafts * a.groups, local = id - s.id0, n = s.rows + s.drafts;
+  const uint32_t R = s.drafts * a.groups, local = id - p.id0[seq], n = s.rows + s.drafts;
   const uint32_t kvh = p.kv0 + local / R, row = local % R, used = (n + p.chunk - 1) / p.chunk;
   const uint32_t wused = (n + p.wchunk - 1) / p.wchunk;
   RowEnd end = p.ends[id];
@@ -1035,24 +1041,18 @@ void for_groups(const TreeArgs& a, const TreeSeq* seqs, uint32_t n, F&& f) {
 // Keys per chunk, in whole granules (at most 16384 keys, which bounds the int32
 // sums and a wave's key tiles): the share of the longest sequence, among some, that
 // ends first when the device runs `want` blocks at a time, each for its chunk and
-// `extra` keys' time besides. Ragged sequences leave a share of the longest one's
-// chunks empty.
-uint32_t chunk_of(const Launch& p, uint64_t keys, uint32_t block_rows, uint32_t dim_blocks, uint64_t want,
-                  uint32_t granule, uint32_t extra) {
-  uint64_t units = 0;
-  for (uint32_t b = 0; b < p.n_seq; ++b) units += (p.s[b].drafts * p.a.groups + block_rows - 1) / block_rows;
-  units *= uint64_t(p.nkv) * dim_blocks;
-  const uint64_t even = std::max<uint64_t>(want / units, 1);
+// `extra` keys' time besides. An item has `per_item` blocks, those past a sequence's
+// own rows too (they wait for a place as the others do).
+uint32_t chunk_of(const Launch& p, uint64_t keys, uint64_t per_item, uint64_t want, uint32_t granule, uint32_t extra) {
+  const uint64_t even = std::max<uint64_t>(want / (p.n_seq * p.nkv * per_item), 1);
   uint64_t best = 0, least = UINT64_MAX, last = 0;
   for (uint64_t n = even; n <= 4 * even; n += (even + 3) / 4) {
     const uint64_t c = std::min<uint64_t>(up((keys + n - 1) / n, granule), 16384 / granule * granule);
     if (c == last) continue;
     last = c;
     uint64_t blocks = 0;
-    for (uint32_t b = 0; b < p.n_seq; ++b)
-      blocks += ((p.s[b].drafts * p.a.groups + block_rows - 1) / block_rows) *
-                ((uint64_t(p.s[b].rows) + p.s[b].drafts + c - 1) / c);
-    blocks *= uint64_t(p.nkv) * dim_blocks;
+    for (uint32_t b = 0; b < p.n_seq; ++b) blocks += (uint64_t(p.s[b].rows) + p.s[b].drafts + c - 1) / c;
+    blocks *= p.nkv * per_item;
     const uint64_t cost = (blocks + want - 1) / want * (std::min(c, keys) + extra);
     if (cost < least) least = cost, best = c;
   }
@@ -1075,7 +1075,8 @@ uint64_t plan(const TreeArgs& a, const TreeSeq* seqs, const Group& g, Launch& p)
   for (uint32_t b = g.b0; b < g.b1; ++b) {
     const TreeSeq& t = seqs[b];
     Seq& s = p.s[b - g.b0];
-    s = {t.k, t.v, t.ld, t.first, t.wrap, t.row0, scores, t.rows, t.drafts, p.rows, score_ld(t)};
+    s = {t.k, t.v, t.ld, t.first, t.wrap, t.row0, scores, t.rows, t.drafts, score_ld(t)};
+    p.id0[b - g.b0] = p.rows;
     if (t.rows) {
       w4 = w4 && t.ld % 4 == 0 && aligned(t.k, 16);
       w2 = w2 && t.ld % 2 == 0 && aligned(t.v, 8);
@@ -1094,7 +1095,7 @@ uint64_t plan(const TreeArgs& a, const TreeSeq* seqs, const Group& g, Launch& p)
   // their sums' registers would leave the device half empty
   p.block_rows = std::min<uint32_t>(uint32_t(up(most, 16)), a.hd <= 256 ? (most > 64 && w4 ? 128 : 64) : 32);
   p.row_blocks = (most + p.block_rows - 1) / p.block_rows;
-  p.chunk = chunk_of(p, keys, p.block_rows, 1, p.block_rows > 64 ? 256 : 512, 16 * kWaves, 256);
+  p.chunk = chunk_of(p, keys, p.row_blocks, p.block_rows > 64 ? 256 : 512, 16 * kWaves, 256);
   p.chunks = uint32_t((keys + p.chunk - 1) / p.chunk);
   // (28 rows of 3000 keys 32 us whole and 34 by chunks, of 6000 39 and 39, of 15000
   // 51 and 46; 160 rows of 15000 84 and 86)
@@ -1103,9 +1104,15 @@ uint64_t plan(const TreeArgs& a, const TreeSeq* seqs, const Group& g, Launch& p)
   p.splits = kWaves / p.groups;
   p.sum_rows = std::min<uint32_t>(uint32_t(up(most, 16)), a.hd <= 64 ? 32 : 64);
   p.sum_blocks = (most + p.sum_rows - 1) / p.sum_rows;
-  p.wchunk = chunk_of(p, keys, p.sum_rows, (a.hd + kSumDims - 1) / kSumDims, 256, 64, 128);
+  p.wchunk = chunk_of(p, keys, uint64_t(p.sum_blocks) * ((a.hd + kSumDims - 1) / kSumDims), 256, 64, 128);
   p.splits = std::min(p.splits, p.wchunk / 64);
   p.wchunks = uint32_t((keys + p.wchunk - 1) / p.wchunk);
+  for (uint32_t b = 0; b < p.n_seq; ++b) {
+    const uint64_t n = uint64_t(p.s[b].rows) + p.s[b].drafts;
+    p.item0[b] = p.items, p.witem0[b] = p.witems;
+    p.items += g.nkv * uint32_t((n + p.chunk - 1) / p.chunk);
+    p.witems += g.nkv * uint32_t((n + p.wchunk - 1) / p.wchunk);
+  }
   uint64_t at = 0;
   auto take = [&](uint64_t bytes) {
     const uint64_t o = at;
@@ -1183,23 +1190,22 @@ void launch_tree_attention(const TreeArgs& a, const TreeSeq* seqs, uint32_t n, v
     };
     place(p.scores), place(p.pmax), place(p.psum), place(p.pfirst), place(p.planes), place(p.pweight);
     place(p.ends), place(p.weights);
-    const uint32_t units = p.n_seq * p.nkv;
-    auto blocks = [&](uint32_t chunks) { return uint32_t(up(uint64_t(units) * chunks, 8)); };
+    const uint32_t score_blocks = uint32_t(up(p.items, 8)) * p.row_blocks, sum_blocks = uint32_t(up(p.witems, 8)) * p.sum_blocks;
     const uint32_t nsub = (a.hd + 63) / 64;
-    if (nsub == 1) launch_scores<1>(p, blocks(p.chunks) * p.row_blocks, s);
-    else if (nsub == 2) launch_scores<2>(p, blocks(p.chunks) * p.row_blocks, s);
-    else if (nsub == 3) launch_scores<3>(p, blocks(p.chunks) * p.row_blocks, s);
-    else if (nsub == 4) launch_scores<4>(p, blocks(p.chunks) * p.row_blocks, s);
-    else launch_scores<8>(p, blocks(p.chunks) * p.row_blocks, s);
+    if (nsub == 1) launch_scores<1>(p, score_blocks, s);
+    else if (nsub == 2) launch_scores<2>(p, score_blocks, s);
+    else if (nsub == 3) launch_scores<3>(p, score_blocks, s);
+    else if (nsub == 4) launch_scores<4>(p, score_blocks, s);
+    else launch_scores<8>(p, score_blocks, s);
     if (p.whole) {
       launch_rows(p, s);
     } else {
       hipLaunchKernelGGL(k_tree_terms, dim3((p.rows + 3) / 4, p.chunks), dim3(256), 0, s, p);
       hipLaunchKernelGGL(k_tree_weights, dim3((p.rows + 3) / 4, p.chunks), dim3(256), 0, s, p);
     }
-    if (p.sum_rows <= 16) launch_wsum<1>(p, blocks(p.wchunks) * p.sum_blocks, s);
-    else if (p.sum_rows <= 32) launch_wsum<2>(p, blocks(p.wchunks) * p.sum_blocks, s);
-    else launch_wsum<4>(p, blocks(p.wchunks) * p.sum_blocks, s);
+    if (p.sum_rows <= 16) launch_wsum<1>(p, sum_blocks, s);
+    else if (p.sum_rows <= 32) launch_wsum<2>(p, sum_blocks, s);
+    else launch_wsum<4>(p, sum_blocks, s);
     if (p.wchunks * p.splits > 16)
       hipLaunchKernelGGL(k_tree_join<4>, dim3(p.rows, (a.hd + 63) / 64), dim3(256), 0, s, p);
     else
